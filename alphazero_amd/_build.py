@@ -8,8 +8,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 SRCS = [os.path.join(_HERE, "csrc", "az_engine.hip"), os.path.join(_HERE, "csrc", "az_tower.hip"),
         os.path.join(_HERE, "csrc", "az_tower_f32.hip"), os.path.join(_HERE, "csrc", "az_smallnet.hip"),
         os.path.join(_HERE, "csrc", "az_tower_h2.hip"), os.path.join(_HERE, "csrc", "az_tower_h1.hip"),
-        os.path.join(_HERE, "csrc", "az_tower_w.hip")]
-DEPS = [*SRCS, os.path.join(_HERE, "csrc", "az_games.hip.h"),
+        os.path.join(_HERE, "csrc", "az_tower_w.hip"), os.path.join(_HERE, "csrc", "az_sample.hip")]
+DEPS = [*SRCS, os.path.join(_HERE, "csrc", "az_games.hip.h"), os.path.join(_HERE, "csrc", "az_ops.hip.h"),
         os.path.join(os.path.dirname(_HERE), "include", "az_engine.h")]
 LIB_DIR = os.path.join(_HERE, "lib")
 # AZ_ENGINE_LIB: load another build of the library instead (A/B measurements of kernel variants: scripts/dev/build_variant.sh)
@@ -19,6 +19,9 @@ LIB = os.environ.get("AZ_ENGINE_LIB") or os.path.join(LIB_DIR, "libaz_engine.so"
 # like the reference's torch-CPU chain (bit-exactness notes).
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=off",
          "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-int-to-void-pointer-cast"]
+# the operator files: no packed f32 arithmetic (some of its forms are not safe on this card)
+OPS_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+OPS_SRCS = ("az_sample.hip", "az_norm.hip", "az_ortho.hip")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")  # per-source objects (git-ignored): only what changed is recompiled
 
 
@@ -41,7 +44,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         objs.append(obj)
         newest = max(os.path.getmtime(f) for f in [src, *headers] if os.path.exists(f))
         if force or not os.path.exists(obj) or os.path.getmtime(obj) < newest:
-            cmd = [hipcc, *FLAGS, "-c", "-o", obj, src]
+            cmd = [hipcc, *FLAGS, *(OPS_FLAGS if os.path.basename(src) in OPS_SRCS else []), "-c", "-o", obj, src]
             if verbose:
                 print(" ".join(cmd))
             jobs.append((cmd, subprocess.Popen(cmd)))

@@ -7,6 +7,10 @@ network B: every move of a game is that AI move made by the network whose turn i
 evaluates every leaf of its own search, as in the UI where one model owns one search), Dirichlet noise off
 by default, ties to the lowest action index as ``argmax`` does on the reference's CPU tensors.
 Games alternate colours: A moves first in even games, B in odd ones.
+
+Deterministic play between two fixed networks is two games however many are asked for; ``opening_plies`` draws the first moves
+of every game from its search's visit counts instead (ops.sample_actions: visits ** (1 / temperature), cut by top_k, top_p and
+min_p), as self-play does at training/self_play.py:73-74.
 """
 from __future__ import annotations
 
@@ -16,17 +20,22 @@ import torch
 
 from .arena import C_PUCT, EPSILON, TRAIN_NUM_SIMULATION, engine_constants, resolve_game
 from .engine import Engine, EngineError
+from .ops import sample_actions
 
 
 @torch.no_grad()
 def play_match(game_cls, model_a: torch.nn.Module, model_b: torch.nn.Module, n_games: int,
                num_simulation: int = TRAIN_NUM_SIMULATION, c_puct: float = C_PUCT,
-               device: Optional[torch.device] = None, record_moves: bool = False, fused: Optional[bool] = False) -> dict:
+               device: Optional[torch.device] = None, record_moves: bool = False, fused: Optional[bool] = False,
+               opening_plies: int = 0, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+               seed: int = 0) -> dict:
     """Returns {"a_wins", "b_wins", "draws", "results" (n_games,) from A's point of view in {+1, 0, -1},
     "plies" (n_games,), and with record_moves "moves": a list of (n_games,) int32 tensors, -1 once a game is over}.
     ``fused``: False = each network's own PyTorch forward on the rows it owns; True / None = the hand-written f32 network
     kernels (alphazero_amd.fused) reading the packed leaf batch, each network evaluating the rows flagged for it (None: only
-    when kernels cover BOTH networks; True: required)."""
+    when kernels cover BOTH networks; True: required).
+    ``opening_plies`` > 0: the moves of a game's first plies are drawn from its visit counts at ``temperature`` (top_k, top_p,
+    min_p: ops.sample_actions) with uniform numbers from a generator seeded with ``seed``; the same seed plays the same match."""
     if not torch.cuda.is_available():
         raise EngineError("play_match needs a GPU (no CPU fallback)")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
@@ -57,6 +66,8 @@ def play_match(game_cls, model_a: torch.nn.Module, model_b: torch.nn.Module, n_g
     a_first = (torch.arange(n_games, device=dev) % 2 == 0)  # A is PLAYER1 (+1, moves first) in even games
     results = torch.zeros(n_games, device=dev)
     ar = torch.arange(A, device=dev)
+    gen = torch.Generator(device=dev).manual_seed(int(seed)) if opening_plies > 0 else None
+    ply = 0  # (all games start together: a game's ply is the round's number)
     moves = []
     eng.reset_games(None)
     while True:
@@ -92,6 +103,11 @@ def play_match(game_cls, model_a: torch.nn.Module, model_b: torch.nn.Module, n_g
         # prior.argmax(dim=1): the most visited action, the lowest index among equals
         top = visits.max(1, keepdim=True).values
         forced = torch.where(visits == top, ar, A).min(1).values.to(torch.int32)
+        if ply < opening_plies:
+            drawn = sample_actions(torch.log(visits.float()), torch.rand(n_games, device=dev, generator=gen), temperature=temperature,
+                                   top_k=top_k, top_p=top_p, min_p=min_p)  # (an unvisited action has the score -inf)
+            forced = torch.where(drawn >= 0, drawn, forced)
+        ply += 1
         forced = torch.where(act, forced, torch.full_like(forced, -1))
         eng.play_moves(ones, expo, forced, actions, done)
         if record_moves:

@@ -440,6 +440,25 @@ int az_tower_heads_forward_static(int32_t board_size, int32_t channels, int32_t 
                                   const void *w1_dev, const float *b1_dev, const float *w2_dev, float b2, float *logits_dev,
                                   float *values_dev, void *stream);
 
+/* ---- operators around a training generation.  Errors through az_tower_last_error(); dtype: AZ_NN_F32 / AZ_NN_BF16 / AZ_NN_F16. ---- */
+
+/* One action per row of scores from a given uniform number; the reference draws from a temperature alone
+ * (training/self_play.py:73-74).  scores_dev (rows, n) of `dtype`, rows row_stride elements apart (0: one row for all draws);
+ * legal_dev NULL or (rows, n) bytes, 0 = the score does not count (nor does NaN or -inf); uniforms_dev (rows) f32 in [0, 1).
+ *   w_i = exp((s_i - max s) / temperature); temperature 0: the first of the largest scores;
+ *   order: s descending, equal scores by ascending index; top_k 0 = all, else the first top_k of the order;
+ *   top_p: members whose mass before them is < top_p of the mass left by top_k (the first always); min_p: w_i >= min_p;
+ *   action = the smallest index whose kept mass up to and including it is > u * the kept mass; -1 where nothing counts.
+ * Rows with scores of +inf share the mass among those.  temperature, top_k, top_p and min_p: one number, or (rows) values
+ * (f32, top_k i32) where the _dev pointer is given (a temperature that is not > 0 counts as 0, a top_k below 1 as all, a top_p
+ * that is not < 1 as 1, a min_p that is not > 0 as 0).  actions_dev (rows) i32; logprobs_dev NULL or (rows) f32: the natural
+ * logarithm of the drawn action's share of the kept mass, -inf beside an action of -1.  1 <= n <= 524,288.  The result does not
+ * depend on the launch: masses are summed as integers. */
+int az_sample_actions(int32_t dtype, int32_t rows, int32_t n, const void *scores_dev, int64_t row_stride, const uint8_t *legal_dev,
+                      int64_t legal_stride, const float *uniforms_dev, const float *temperature_dev, double temperature,
+                      const int32_t *top_k_dev, int32_t top_k, const float *top_p_dev, double top_p, const float *min_p_dev,
+                      double min_p, int32_t *actions_dev, float *logprobs_dev, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
