@@ -89,13 +89,65 @@ class _Res(nn.Module):
         return self._relu(y + x)
 
 
-class GomokuNet(DualHeadNet):
-    """ResNet tower; defaults = the reference GomokuModel (15x15, 64 ch, 2 blocks, 233,257 params)."""
+class GroupNormAct(nn.Module):
+    """group norm + activation (+ a residual sum before it) over channels-last samples as one operator
+    (alphazero_amd.ops.group_norm_act: HIP kernels, forward and backward; GPU tensors only).  Parameter names follow
+    nn.GroupNorm; ``forward(x, residual=None)``."""
 
-    def __init__(self, board_size: int = 15, channels: int = 64, blocks: int = 2, history_len: int = HISTORY_LEN) -> None:
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, activation: str = "relu") -> None:
+        super().__init__()
+        if num_channels % num_groups:
+            raise ValueError("num_channels must be a multiple of num_groups")
+        self.num_groups, self.num_channels, self.eps, self.activation = num_groups, num_channels, eps, activation
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x, residual=None):
+        from .ops import group_norm_act
+
+        return group_norm_act(x, self.num_groups, self.weight, self.bias, eps=self.eps, activation=self.activation, residual=residual)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, activation={self.activation!r}"
+
+
+class _GroupRes(nn.Module):
+    """``_Res`` with group norm: the block's sum and last activation belong to its second norm"""
+
+    def __init__(self, c: int, groups: int) -> None:
+        super().__init__()
+        self._conv1 = nn.Conv2d(c, c, 3, padding=1, bias=False)
+        self._gn1 = GroupNormAct(groups, c)
+        self._conv2 = nn.Conv2d(c, c, 3, padding=1, bias=False)
+        self._gn2 = GroupNormAct(groups, c)
+
+    def forward(self, x):
+        return self._gn2(self._conv2(self._gn1(self._conv1(x))), residual=x)
+
+
+class GomokuNet(DualHeadNet):
+    """ResNet tower; defaults = the reference GomokuModel (15x15, 64 ch, 2 blocks, 233,257 params).
+
+    ``norm="group"``: every BatchNorm2d + ReLU becomes a GroupNormAct (``groups`` groups of the trunk's channels, one group in the
+    heads).  Such a net has no running statistics: training and evaluation are one function, and the ranks of a data-parallel run
+    hold nothing that drifts apart between weight broadcasts.  It runs through its own forward (on the GPU, in channels-last memory),
+    not on the fused towers, which fold BatchNorm into their convolutions."""
+
+    def __init__(self, board_size: int = 15, channels: int = 64, blocks: int = 2, history_len: int = HISTORY_LEN, norm: str = "batch",
+                 groups: int = 8) -> None:
         super().__init__()
         a = board_size * board_size
         self.board_size = board_size
+        if norm not in ("batch", "group"):
+            raise ValueError("norm: 'batch' or 'group'")
+        if norm == "group":
+            self._shared_layers = nn.Sequential(
+                nn.Conv2d(history_len + 1, channels, 3, padding=1, bias=False), GroupNormAct(groups, channels),
+                *[_GroupRes(channels, groups) for _ in range(blocks)])
+            self._policy_head = nn.Sequential(nn.Conv2d(channels, 1, 1, bias=False), GroupNormAct(1, 1), nn.Flatten(1), nn.Linear(a, a))
+            self._value_head = nn.Sequential(nn.Conv2d(channels, 2, 1, bias=False), GroupNormAct(1, 2), nn.Flatten(1), *_mlp_value(2 * a))
+            self.to(memory_format=torch.channels_last)
+            return
         self._shared_layers = nn.Sequential(
             nn.Conv2d(history_len + 1, channels, 3, padding=1, bias=False), nn.BatchNorm2d(channels), nn.ReLU(),
             *[_Res(channels) for _ in range(blocks)])

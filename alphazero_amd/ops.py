@@ -1,5 +1,5 @@
 """Operators around a training generation, as hand-written HIP kernels behind the C ABI (include/az_engine.h): choosing moves from
-scores (``sample_actions``).
+scores (``sample_actions``) and the normalisation layer of a residual tower with its gradient (``group_norm_act``).
 
 Tensors live on the GPU; every call is asynchronous on torch's current stream of the tensors' device and may be captured into a
 HIP graph.  There is no CPU path: a tensor elsewhere, or a shape or type a kernel does not cover, raises ``EngineError``."""
@@ -84,3 +84,97 @@ def sample_actions(scores: torch.Tensor, uniforms: torch.Tensor, *, temperature=
             _ptr(uniforms), _ptr(t_t), float(t_v), _ptr(k_t), min(int(k_v), n), _ptr(p_t), float(p_v), _ptr(m_t), float(m_v),
             _ptr(actions), _ptr(logp), _stream(dev)))
     return (actions, logp) if return_logprobs else actions
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """the tensor as dense channels-last samples (a copy where it is not)"""
+    return t.contiguous(memory_format=torch.channels_last)
+
+
+def _empty_like(x: torch.Tensor) -> torch.Tensor:
+    n, c, h, w = x.shape
+    return torch.empty((n, h, w, c), dtype=x.dtype, device=x.device).permute(0, 3, 1, 2)
+
+
+def _workspace(backward: int, n: int, hw: int, c: int, groups: int, device) -> torch.Tensor:
+    size = load_library().az_group_norm_workspace(backward, n, hw, c, groups)
+    if size < 0:
+        _check(-1)
+    return torch.empty(max(int(size), 16), dtype=torch.uint8, device=device)
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, groups, eps, act):
+        n, c, h, w = x.shape
+        x = _dense(x)
+        residual = _dense(residual) if residual is not None else None
+        weight = weight.contiguous() if weight is not None else None
+        bias = bias.contiguous() if bias is not None else None
+        pd = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        with torch.cuda.device(x.device):
+            y = _empty_like(x)
+            stats = torch.empty((n, groups, 2), dtype=torch.float64, device=x.device)
+            ws = _workspace(0, n, h * w, c, groups, x.device)
+            _check(load_library().az_group_norm_forward(
+                _NN_DTYPES[x.dtype], _NN_DTYPES[pd], n, h * w, c, groups, act, float(eps), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias),
+                _ptr(y), _ptr(stats), _ptr(ws), ws.numel(), _stream(x.device)))
+        ctx.save_for_backward(x, weight, bias, residual, stats)
+        ctx.groups, ctx.act, ctx.pd = groups, act, pd
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, residual, stats = ctx.saved_tensors
+        n, c, h, w = x.shape
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dy = _dense(dy)
+        with torch.cuda.device(x.device):
+            dx = _empty_like(x) if need_x else None
+            dw = torch.empty(c, dtype=ctx.pd, device=x.device) if need_w else None
+            db = torch.empty(c, dtype=ctx.pd, device=x.device) if need_b else None
+            dr = _empty_like(x) if need_r and ctx.act else None
+            ws = _workspace(1, n, h * w, c, ctx.groups, x.device)
+            if need_x or need_w or need_b or dr is not None:
+                _check(load_library().az_group_norm_backward(
+                    _NN_DTYPES[x.dtype], _NN_DTYPES[ctx.pd], n, h * w, c, ctx.groups, ctx.act, _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias),
+                    _ptr(dy), _ptr(stats), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream(x.device)))
+        if need_r and dr is None:
+            dr = dy  # (no activation: the sum passes the gradient on)
+        return dx, dw, db, dr, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                   eps: float = 1e-5, activation: str = "relu", residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(group_norm(x) * weight + bias (+ residual))`` with its gradient, for x (N, C, H, W) f32 / bf16 / f16 whose memory is
+    channels last (other layouts are copied into it first; the result is channels last).  ``activation``: "none", "relu" or
+    "silu".  weight and bias (C,) are f32 or of x's dtype, both alike; ``residual`` is like x.  Statistics are held in f64, the
+    rest in f32, and each output is rounded once.  Differentiable once, in every tensor argument."""
+    _on_gpu(x, "x", tuple(_NN_DTYPES))
+    if x.dim() != 4:
+        raise EngineError(f"x: expected (N, C, H, W), got {tuple(x.shape)}")
+    n, c, h, w = x.shape
+    if activation not in ACTIVATIONS:
+        raise EngineError(f"activation: one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    if not isinstance(num_groups, int) or num_groups < 1 or c < 1 or c % num_groups or c > 16384 or num_groups > 1024:
+        raise EngineError(f"{c} channels in {num_groups} groups: expected 1 .. 16,384 channels, a multiple of 1 .. 1,024 groups")
+    if n > 1 << 28 or h * w > 1 << 28:
+        raise EngineError("at most 2^28 samples of 2^28 pixels")
+    if not eps >= 0.0:
+        raise EngineError("eps >= 0")
+    dtypes = {x.dtype, torch.float32}
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _on_gpu(t, name, tuple(dtypes), x.device)
+            if tuple(t.shape) != (c,):
+                raise EngineError(f"{name}: expected ({c},), got {tuple(t.shape)}")
+            dtypes = {t.dtype}  # (the second one like the first)
+    if residual is not None:
+        _on_gpu(residual, "residual", (x.dtype,), x.device)
+        if residual.shape != x.shape:
+            raise EngineError(f"residual: expected {tuple(x.shape)}, got {tuple(residual.shape)}")
+    return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, ACTIVATIONS[activation])

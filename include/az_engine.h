@@ -459,6 +459,30 @@ int az_sample_actions(int32_t dtype, int32_t rows, int32_t n, const void *scores
                       const int32_t *top_k_dev, int32_t top_k, const float *top_p_dev, double top_p, const float *min_p_dev,
                       double min_p, int32_t *actions_dev, float *logprobs_dev, void *stream);
 
+#define AZ_ACT_NONE 0
+#define AZ_ACT_RELU 1
+#define AZ_ACT_SILU 2
+
+/* Group norm with an activation over channels-last samples, and its gradient (the reference's networks normalise with BatchNorm2d:
+ * nn_models/resnet_blocks.py:28-40; group norm needs no statistics shared between ranks).
+ *   x_dev (n, hw, c) of `dtype`, dense; group g = channels g * c/groups .. ; mean and variance (divided by hw * c/groups) of a
+ *   sample's group; z = (x - mean) / sqrt(var + eps) * weight + bias (+ residual), y = act(z).
+ * weight_dev / bias_dev (c) or NULL (1 / 0) of param_dtype (AZ_NN_F32 or `dtype`); residual_dev NULL or like x; y_dev like x;
+ * stats_dev (n, groups, 2) f64 out: mean and 1/sqrt(var + eps), what the backward call reads.
+ * Backward: dy_dev like x; dx_dev, dresidual_dev like x, dweight_dev, dbias_dev (c) of param_dtype, each may be NULL (not wanted).
+ *   relu's derivative at 0 is 0.  n * hw = 0: nothing is written but zero dweight / dbias.
+ * workspace_dev: az_group_norm_workspace() bytes (backward 0 / 1; -1: refused), aligned to 16 bytes, meaningless between calls; calls that
+ * overlap in time need one each.  c at most 16,384, at most 1,024 groups, 2^28 samples, 2^28 pixels.  No output may overlap an input
+ * or another output.  The result does not depend on timing: sums are taken in a fixed order. */
+int64_t az_group_norm_workspace(int32_t backward, int64_t n, int64_t hw, int32_t c, int32_t groups);
+int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t groups, int32_t act, double eps,
+                          const void *x_dev, const void *residual_dev, const void *weight_dev, const void *bias_dev, void *y_dev,
+                          double *stats_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
+int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t groups, int32_t act,
+                           const void *x_dev, const void *residual_dev, const void *weight_dev, const void *bias_dev, const void *dy_dev,
+                           const double *stats_dev, void *dx_dev, void *dresidual_dev, void *dweight_dev, void *dbias_dev,
+                           void *workspace_dev, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -63,3 +63,63 @@ def test_sample_python_refusals_on_the_gpu():
                 lambda: ops.sample_actions(s, u, top_p=torch.ones(3, device="cuda")), lambda: ops.sample_actions(s, u, top_k=torch.ones(2, device="cuda"))):
         with pytest.raises(EngineError):
             bad()
+
+
+def _norm(lib, backward=False, **kw):
+    a = dict(dtype=0, pd=0, n=2, hw=9, c=8, g=2, act=1, eps=1e-5, x=64, r=None, w=None, b=None, dy=64, y=64, stats=64, ws=64, size=1 << 20)
+    a.update(kw)
+    if backward:
+        return lib.az_group_norm_backward(a["dtype"], a["pd"], a["n"], a["hw"], a["c"], a["g"], a["act"], a["x"], a["r"], a["w"], a["b"], a["dy"],
+                                          a["stats"], a["y"], None, None, None, a["ws"], a["size"], None)
+    return lib.az_group_norm_forward(a["dtype"], a["pd"], a["n"], a["hw"], a["c"], a["g"], a["act"], a["eps"], a["x"], a["r"], a["w"], a["b"], a["y"],
+                                     a["stats"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(pd=1), dict(dtype=1, pd=2), dict(act=3), dict(act=-1), dict(n=-1), dict(hw=-1), dict(c=0), dict(g=0),
+                                 dict(g=3), dict(c=16385, g=1), dict(c=2048, g=2048), dict(n=(1 << 28) + 1), dict(hw=(1 << 28) + 1), dict(x=None),
+                                 dict(stats=None), dict(ws=None), dict(size=16), dict(x=66), dict(dtype=1, pd=1, w=65), dict(stats=68), dict(r=65)])
+def test_norm_refuses(bad, backward):
+    lib = _lib()
+    assert _norm(lib, backward, **bad) == -1
+    assert lib.az_tower_last_error().startswith(b"group norm:")
+
+
+def test_norm_sizes():
+    lib = _lib()
+    assert _norm(lib, n=0) == 0 and _norm(lib, hw=0) == 0
+    assert lib.az_group_norm_workspace(0, 4, 81, 64, 5) == -1
+    assert lib.az_group_norm_workspace(0, 0, 81, 64, 8) == 0
+    assert lib.az_group_norm_workspace(1, 4, 81, 64, 8) > 0
+
+
+def test_norm_python_refusals():
+    from alphazero_amd import ops
+    from alphazero_amd.engine import EngineError
+    from alphazero_amd.nets import GomokuNet, GroupNormAct
+
+    with pytest.raises(EngineError, match="no CPU path"):
+        ops.group_norm_act(torch.zeros(2, 8, 3, 3), 2)
+    with pytest.raises(EngineError, match="no CPU path"):
+        GroupNormAct(2, 8)(torch.zeros(2, 8, 3, 3))
+    with pytest.raises(EngineError, match="dtype"):
+        ops.group_norm_act(torch.zeros(2, 8, 3, 3, dtype=torch.float64), 2)
+    with pytest.raises(ValueError):
+        GroupNormAct(3, 8)
+    with pytest.raises(ValueError):
+        GomokuNet(9, 16, 1, norm="layer")
+
+
+@pytest.mark.gpu
+def test_norm_python_refusals_on_the_gpu():
+    from alphazero_amd import ops
+    from alphazero_amd.engine import EngineError
+
+    x, w = torch.zeros(2, 8, 3, 3, device="cuda"), torch.ones(8, device="cuda")
+    for bad in (lambda: ops.group_norm_act(x[0], 2), lambda: ops.group_norm_act(x, 3), lambda: ops.group_norm_act(x, 0), lambda: ops.group_norm_act(x, 2.0),
+                lambda: ops.group_norm_act(x, 2, w[:4]), lambda: ops.group_norm_act(x, 2, w, w.half()), lambda: ops.group_norm_act(x.half(), 2, w.bfloat16()),
+                lambda: ops.group_norm_act(x, 2, w.cpu()), lambda: ops.group_norm_act(x, 2, activation="gelu"), lambda: ops.group_norm_act(x, 2, eps=-1.0),
+                lambda: ops.group_norm_act(x, 2, residual=x.half()), lambda: ops.group_norm_act(x, 2, residual=x[:1]),
+                lambda: ops.group_norm_act(x, 2, eps=float("nan"))):
+        with pytest.raises(EngineError):
+            bad()
