@@ -9,7 +9,7 @@ SRCS = [os.path.join(_HERE, "csrc", "az_engine.hip"), os.path.join(_HERE, "csrc"
         os.path.join(_HERE, "csrc", "az_tower_f32.hip"), os.path.join(_HERE, "csrc", "az_smallnet.hip"),
         os.path.join(_HERE, "csrc", "az_tower_h2.hip"), os.path.join(_HERE, "csrc", "az_tower_h1.hip"),
         os.path.join(_HERE, "csrc", "az_tower_w.hip"), os.path.join(_HERE, "csrc", "az_sample.hip"),
-        os.path.join(_HERE, "csrc", "az_norm.hip")]
+        os.path.join(_HERE, "csrc", "az_norm.hip"), os.path.join(_HERE, "csrc", "az_ortho.hip")]
 DEPS = [*SRCS, os.path.join(_HERE, "csrc", "az_games.hip.h"), os.path.join(_HERE, "csrc", "az_ops.hip.h"),
         os.path.join(os.path.dirname(_HERE), "include", "az_engine.h")]
 LIB_DIR = os.path.join(_HERE, "lib")

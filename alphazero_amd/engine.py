@@ -48,7 +48,8 @@ EXPORTS = ["az_create", "az_destroy", "az_get_dims", "az_last_error", "az_check"
            "az_select_wave", "az_expand_wave", "az_search_remaining", "az_set_virtual_loss", "az_smallnet_forward_f32",
            "az_quick_tower_forward_f32", "az_quick_heads_forward_f32", "az_quick_stash_bytes", "az_quick_tower_forward", "az_quick_heads_forward",
            "az_smallnet_head_floats", "az_draw_rng", "az_philox4x32_10", "az_tower_forward_h2", "az_tower_forward_h1", "az_tower_forward_f32w",
-           "az_sample_actions", "az_group_norm_workspace", "az_group_norm_forward", "az_group_norm_backward"]
+           "az_sample_actions", "az_group_norm_workspace", "az_group_norm_forward", "az_group_norm_backward",
+           "az_orthogonalize_workspace", "az_orthogonalize"]
 
 _lib = None
 
@@ -122,11 +123,15 @@ def load_library() -> C.CDLL:
     lib.az_group_norm_workspace.restype = C.c_int64
     lib.az_group_norm_forward.argtypes = [C.c_int32] * 2 + [C.c_int64] * 2 + [C.c_int32] * 3 + [C.c_double] + [vp] * 7 + [C.c_int64, vp]
     lib.az_group_norm_backward.argtypes = [C.c_int32] * 2 + [C.c_int64] * 2 + [C.c_int32] * 3 + [vp] * 11 + [C.c_int64, vp]
+    lib.az_orthogonalize_workspace.argtypes = [C.c_int32, C.c_int32, vp, vp]
+    lib.az_orthogonalize_workspace.restype = C.c_int64
+    lib.az_orthogonalize.argtypes = [C.c_int32, C.c_int32, vp, vp, vp, vp, C.c_int32] + [C.c_double] * 4 + [vp, C.c_int64, vp]
     lib.az_tower_last_error.argtypes = []
     lib.az_tower_last_error.restype = C.c_char_p
     for name in EXPORTS:
         if name not in ("az_last_error", "az_tower_last_error", "az_heads_feat_stride", "az_static_max_boards",
-                        "az_smallnet_head_floats", "az_quick_stash_bytes", "az_group_norm_workspace"):
+                        "az_smallnet_head_floats", "az_quick_stash_bytes", "az_group_norm_workspace",
+                        "az_orthogonalize_workspace"):
             getattr(lib, name).restype = C.c_int
     _lib = lib
     return lib

@@ -29,6 +29,77 @@ def train_step(model: torch.nn.Module, optim: torch.optim.Optimizer, pool, batch
     return float(loss.detach()), float(pl), float(vl)
 
 
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised (ops.orthogonalize) for every parameter of two or more dimensions, taken as the matrix
+    (shape[0], rest); parameters of one dimension (biases, norms) take AdamW steps.  The reference trains with Adam
+    (training/nn_trainer.py:36-94).  Parameters live on the GPU; all matrices of a type go through one call per step.
+
+        buf <- lerp(buf, g, 1 - momentum);  u = lerp(g, buf, momentum) (nesterov) or buf
+        p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) orthogonalize(u)"""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, steps: int = 5, weight_decay: float = 0.0,
+                 adam_lr: float = 1e-3, betas=(0.9, 0.999), adam_eps: float = 1e-8):
+        if not (lr >= 0 and adam_lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("Muon: lr, adam_lr and weight_decay >= 0; momentum and betas in [0, 1)")
+        params = list(params)
+        common = dict(weight_decay=weight_decay)
+        groups = [dict(params=[p for p in params if p.dim() >= 2], kind="matrix", lr=lr, momentum=momentum, nesterov=nesterov, steps=steps, **common),
+                  dict(params=[p for p in params if p.dim() < 2], kind="vector", lr=adam_lr, betas=tuple(betas), eps=adam_eps, **common)]
+        super().__init__([g for g in groups if g["params"]], dict(lr=lr))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_type: dict = {}
+            for p in group["params"]:
+                if p.grad is not None and p.numel():
+                    by_type.setdefault((p.device, p.dtype), []).append(p)
+            for ps in by_type.values():
+                (self._matrices if group["kind"] == "matrix" else self._vectors)(group, ps)
+        return loss
+
+    def _matrices(self, group, ps) -> None:
+        from .ops import orthogonalize
+
+        grads = [p.grad for p in ps]
+        for p in ps:
+            if "momentum" not in self.state[p]:
+                self.state[p]["momentum"] = torch.zeros_like(p)
+        bufs = [self.state[p]["momentum"] for p in ps]
+        m = group["momentum"]
+        torch._foreach_lerp_(bufs, grads, 1 - m)
+        us = torch._foreach_lerp(grads, bufs, m) if group["nesterov"] else bufs
+        us = orthogonalize([u.reshape(u.shape[0], -1) for u in us], steps=group["steps"])
+        if group["weight_decay"]:
+            torch._foreach_mul_(ps, 1 - group["lr"] * group["weight_decay"])
+        scale = [-group["lr"] * max(1.0, u.shape[0] / u.shape[1]) ** 0.5 for u in us]
+        torch._foreach_mul_(us, scale)
+        torch._foreach_add_(ps, [u.view(p.shape) for u, p in zip(us, ps)])
+
+    def _vectors(self, group, ps) -> None:
+        b1, b2 = group["betas"]
+        for p in ps:
+            st = self.state[p]
+            if "step" not in st:
+                st.update(step=0, exp_avg=torch.zeros_like(p), exp_avg_sq=torch.zeros_like(p))
+            st["step"] += 1
+        grads, avg, sq = [p.grad for p in ps], [self.state[p]["exp_avg"] for p in ps], [self.state[p]["exp_avg_sq"] for p in ps]
+        torch._foreach_lerp_(avg, grads, 1 - b1)
+        torch._foreach_mul_(sq, b2)
+        torch._foreach_addcmul_(sq, grads, grads, 1 - b2)
+        if group["weight_decay"]:
+            torch._foreach_mul_(ps, 1 - group["lr"] * group["weight_decay"])
+        den = torch._foreach_sqrt(sq)
+        torch._foreach_div_(den, [(1 - b2 ** self.state[p]["step"]) ** 0.5 for p in ps])
+        torch._foreach_add_(den, group["eps"])
+        num = torch._foreach_div(avg, [1 - b1 ** self.state[p]["step"] for p in ps])
+        torch._foreach_addcdiv_(ps, num, den, -group["lr"])
+
+
 class DataParallelLearner:
     """``train_step`` on every rank's own batch with the gradients averaged across ranks (BASELINE
     config 5): one process per GPU, ``torch.distributed`` (backend "nccl" = RCCL over xGMI; "gloo" in the CPU tests).

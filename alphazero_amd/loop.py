@@ -18,7 +18,7 @@ import torch
 
 from .arena import SelfPlayRunner, reference_tao
 from .engine import Engine
-from .learner import DataParallelLearner
+from .learner import DataParallelLearner, Muon
 from .samples import DeviceSampleRing, WeightPublisher
 
 UPDATE_MODEL_FREQUENCY = 300  # config/train_config.py:28 (train steps between publishes)
@@ -27,16 +27,21 @@ UPDATE_MODEL_FREQUENCY = 300  # config/train_config.py:28 (train steps between p
 class SelfPlayTrainLoop:
     def __init__(self, model: torch.nn.Module, game: int, board_size: int, n_slots: int, num_sims: int,
                  device: torch.device, *, ring_capacity: int = 1 << 18, batch_size: int = 512,
-                 train_steps_per_move: int = 1, min_samples: int = 4096, lr: float = 1e-3,
+                 train_steps_per_move: int = 1, min_samples: int = 4096, lr: Optional[float] = None, optimizer: str = "adam",
                  nn_dtype: torch.dtype = torch.bfloat16, fused: Optional[bool] = None,
                  publish_every: int = UPDATE_MODEL_FREQUENCY, force_collectives: bool = False,
                  engine=None, runner=None, ring=None):
         """engine / runner / ring: prebuilt parts (the CPU tests of the multi-rank control flow hand in stand-ins that
-        need no GPU); by default they are built here from the other arguments."""
+        need no GPU); by default they are built here from the other arguments.
+        optimizer: "adam" (lr 1e-3 unless given) or "muon" (learner.Muon: orthogonalised updates of the weight matrices, lr 0.02 unless
+        given, Adam's 1e-3 for biases and norms)."""
+        if optimizer not in ("adam", "muon"):
+            raise ValueError("optimizer: 'adam' or 'muon'")
         self.device = device
         self.force_collectives = force_collectives
         self.master = model.to(device).float()  # the learner's f32 weights
-        self.optim = torch.optim.Adam(self.master.parameters(), lr=lr)
+        self.optim = torch.optim.Adam(self.master.parameters(), lr=1e-3 if lr is None else lr) if optimizer == "adam" else \
+            Muon(self.master.parameters(), lr=0.02 if lr is None else lr)
         self.learner = DataParallelLearner(self.master, self.optim, force_collectives=force_collectives)
         self.publisher = WeightPublisher(self.master, src=0)
         self.publisher.publish(force=force_collectives)  # every rank starts from rank 0's weights

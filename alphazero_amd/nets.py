@@ -146,7 +146,6 @@ class GomokuNet(DualHeadNet):
                 *[_GroupRes(channels, groups) for _ in range(blocks)])
             self._policy_head = nn.Sequential(nn.Conv2d(channels, 1, 1, bias=False), GroupNormAct(1, 1), nn.Flatten(1), nn.Linear(a, a))
             self._value_head = nn.Sequential(nn.Conv2d(channels, 2, 1, bias=False), GroupNormAct(1, 2), nn.Flatten(1), *_mlp_value(2 * a))
-            self.to(memory_format=torch.channels_last)
             return
         self._shared_layers = nn.Sequential(
             nn.Conv2d(history_len + 1, channels, 3, padding=1, bias=False), nn.BatchNorm2d(channels), nn.ReLU(),

@@ -1,5 +1,6 @@
 """Operators around a training generation, as hand-written HIP kernels behind the C ABI (include/az_engine.h): choosing moves from
-scores (``sample_actions``) and the normalisation layer of a residual tower with its gradient (``group_norm_act``).
+scores (``sample_actions``), the normalisation layer of a residual tower with its gradient (``group_norm_act``) and the orthogonalised
+weight update (``orthogonalize``).
 
 Tensors live on the GPU; every call is asynchronous on torch's current stream of the tensors' device and may be captured into a
 HIP graph.  There is no CPU path: a tensor elsewhere, or a shape or type a kernel does not cover, raises ``EngineError``."""
@@ -178,3 +179,47 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         if residual.shape != x.shape:
             raise EngineError(f"residual: expected {tuple(x.shape)}, got {tuple(residual.shape)}")
     return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, ACTIVATIONS[activation])
+
+
+@torch.no_grad()
+def orthogonalize(matrices, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+    """Newton-Schulz orthogonalisation: ``X = M / (|M|_F + eps)``, then ``steps`` times ``A = X X^T; X = a X + (b A + c A A) X`` on
+    the shorter side, which moves every singular value towards 1 (with these coefficients, into about 0.7 .. 1.2).
+
+    ``matrices``: a tensor (rows, cols), a batch (n, rows, cols), or a sequence of (rows, cols) tensors of any sizes, all f32, all
+    bf16 or all f16, on one GPU -> new dense tensors of the same shapes and type (a sequence gives a list).  A whole network's
+    matrices in one call cost little more launches than one.  f32 and f16 results are accurate to f32 arithmetic, bf16 ones to
+    about their own rounding.  A matrix that holds an infinity or a NaN gives NaN.  Not differentiable."""
+    single = isinstance(matrices, torch.Tensor)
+    if single and matrices.dim() not in (2, 3):
+        raise EngineError(f"matrices: expected (rows, cols) or (n, rows, cols), got {tuple(matrices.shape)}")
+    if not single and not isinstance(matrices, (list, tuple)):
+        raise EngineError(f"matrices: expected a tensor or a sequence of tensors, got {type(matrices).__name__}")
+    ms = list(matrices) if not single else [matrices] if matrices.dim() == 2 else list(matrices.unbind(0))
+    if not isinstance(steps, int) or not 1 <= steps <= 64:
+        raise EngineError("steps: 1 .. 64")
+    try:
+        a, b, c = (float(v) for v in coefficients)
+    except (TypeError, ValueError) as exc:
+        raise EngineError("coefficients: three numbers") from exc
+    if single:
+        _on_gpu(matrices, "matrices", tuple(_NN_DTYPES))
+    for i, m in enumerate(ms):
+        _on_gpu(m, f"matrices[{i}]", tuple(_NN_DTYPES) if i == 0 else (ms[0].dtype,), ms[0].device if isinstance(ms[0], torch.Tensor) and i else None)
+        if m.dim() != 2 or max(m.shape) > 65536:
+            raise EngineError(f"matrices[{i}]: expected (rows, cols) with sides up to 65,536, got {tuple(m.shape)}")
+    if not ms:
+        return torch.empty_like(matrices) if single else []
+    lib, dev, n = load_library(), ms[0].device, len(ms)
+    with torch.cuda.device(dev):
+        src = [m.contiguous() for m in ms]
+        out = torch.empty(matrices.shape, dtype=matrices.dtype, device=dev) if single else [torch.empty(m.shape, dtype=m.dtype, device=dev) for m in ms]
+        dst = out if not single else [out] if matrices.dim() == 2 else list(out.unbind(0))
+        dt, rows, cols = _NN_DTYPES[ms[0].dtype], (C.c_int32 * n)(*[m.shape[0] for m in ms]), (C.c_int32 * n)(*[m.shape[1] for m in ms])
+        size = lib.az_orthogonalize_workspace(dt, n, rows, cols)
+        if size < 0:
+            _check(-1)
+        ws = torch.empty(max(int(size), 256), dtype=torch.uint8, device=dev)
+        _check(lib.az_orthogonalize(dt, n, (C.c_void_p * n)(*[m.data_ptr() for m in src]), (C.c_void_p * n)(*[m.data_ptr() for m in dst]),
+                                    rows, cols, steps, a, b, c, float(eps), _ptr(ws), ws.numel(), _stream(dev)))
+    return out

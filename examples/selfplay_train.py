@@ -28,6 +28,8 @@ def main():
     ap.add_argument("--board", type=int, default=15, choices=[9, 15])
     ap.add_argument("--batch", type=int, default=1024)
     ap.add_argument("--train-steps-per-move", type=int, default=4)
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"], help="muon: orthogonalised updates (alphazero_amd.learner.Muon)")
+    ap.add_argument("--norm", default="batch", choices=["batch", "group"], help="group: GroupNormAct layers (gomoku net; plays through its own forward)")
     args = ap.parse_args()
     import torch
     import torch.distributed as dist
@@ -45,9 +47,9 @@ def main():
     if args.net == "quick":
         net, dt_ = QuickNet(args.board, 9, args.channels, args.blocks or 4, args.layers), torch.float32
     else:
-        net, dt_ = GomokuNet(args.board, args.channels, args.blocks or 10), torch.bfloat16
+        net, dt_ = GomokuNet(args.board, args.channels, args.blocks or 10, norm=args.norm), torch.bfloat16
     loop = SelfPlayTrainLoop(net, 2, args.board, args.slots, args.sims, dev, batch_size=args.batch,
-                             train_steps_per_move=args.train_steps_per_move, nn_dtype=dt_)
+                             train_steps_per_move=args.train_steps_per_move, nn_dtype=dt_, optimizer=args.optimizer)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     out = None

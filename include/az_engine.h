@@ -483,6 +483,19 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
                            const double *stats_dev, void *dx_dev, void *dresidual_dev, void *dweight_dev, void *dbias_dev,
                            void *workspace_dev, int64_t workspace_bytes, void *stream);
 
+/* Orthogonalising updates by Newton-Schulz products, many matrices in one call (no counterpart in the reference, whose trainer uses
+ * Adam: training/nn_trainer.py:36-94):
+ *   X = M / (|M|_F + eps), on the shorter side;  `steps` times:  A = X X^T,  X = a X + (b A + c A^2) X;  out = X
+ * in / out: HOST arrays of `count` device pointers, row-major dense matrices of `dtype` with rows[i] x cols[i] elements (a side of 0:
+ * nothing to do; at most 65,536); out[i] may be in[i].  f32 and f16 matrices are computed to f32 accuracy (each factor in two f16
+ * halves), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
+ * under which a singular value in [0, 1] could grow beyond 7.5 are refused.
+ * workspace_dev: az_orthogonalize_workspace() bytes (-1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
+ * time need one each.  Matrices are independent: a matrix's result does not depend on the others in the call. */
+int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols);
+int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols,
+                     int32_t steps, double a, double b, double c, double eps, void *workspace_dev, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

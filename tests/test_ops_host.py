@@ -123,3 +123,60 @@ def test_norm_python_refusals_on_the_gpu():
                 lambda: ops.group_norm_act(x, 2, eps=float("nan"))):
         with pytest.raises(EngineError):
             bad()
+
+
+def _ortho(lib, **kw):
+    a = dict(dtype=0, count=1, ins=[512], outs=[512], rows=[4], cols=[5], steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, ws=512, size=1 << 24)
+    a.update(kw)
+    n = len(a["ins"])
+    return lib.az_orthogonalize(a["dtype"], a["count"], (C.c_void_p * n)(*a["ins"]), (C.c_void_p * n)(*a["outs"]), (C.c_int32 * n)(*a["rows"]),
+                                (C.c_int32 * n)(*a["cols"]), a["steps"], a["a"], a["b"], a["c"], a["eps"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=7), dict(count=-1), dict(rows=[-1]), dict(cols=[65537]), dict(steps=0), dict(steps=65), dict(eps=-1.0),
+                                 dict(eps=float("nan")), dict(a=3.0, b=0.0, c=0.0), dict(a=float("nan")), dict(c=50.0), dict(ins=[None]), dict(outs=[None]),
+                                 dict(ins=[514]), dict(dtype=1, outs=[513]), dict(ws=None), dict(ws=128), dict(size=100)])
+def test_ortho_refuses(bad):
+    lib = _lib()
+    assert _ortho(lib, **bad) == -1
+    assert lib.az_tower_last_error().startswith(b"orthogonalize:")
+
+
+def test_ortho_of_nothing():
+    lib = _lib()
+    assert _ortho(lib, rows=[0]) == 0
+    assert lib.az_orthogonalize(0, 0, None, None, None, None, 5, 3.4445, -4.775, 2.0315, 1e-7, None, 0, None) == 0
+    assert lib.az_orthogonalize_workspace(0, 1, (C.c_int32 * 1)(-1), (C.c_int32 * 1)(1)) == -1
+    assert lib.az_orthogonalize_workspace(0, 1, (C.c_int32 * 1)(0), (C.c_int32 * 1)(9)) == 0
+
+
+def test_ortho_python_refusals():
+    from alphazero_amd import ops
+    from alphazero_amd.engine import EngineError
+    from alphazero_amd.learner import Muon
+
+    for bad in (torch.zeros(3, 4), [torch.zeros(3, 4)], torch.zeros(3), torch.zeros(2, 2, 2, 2), "m", [1.0], torch.zeros(3, 4, dtype=torch.float64)):
+        with pytest.raises(EngineError):
+            ops.orthogonalize(bad)
+    with pytest.raises(EngineError, match="steps"):
+        ops.orthogonalize([], steps=0)
+    with pytest.raises(EngineError, match="coefficients"):
+        ops.orthogonalize([], coefficients=(1.0, 2.0))
+    with pytest.raises(ValueError):
+        Muon([torch.nn.Parameter(torch.zeros(2, 2))], momentum=1.0)
+    p = torch.nn.Parameter(torch.zeros(2, 2))
+    p.grad = torch.ones(2, 2)
+    with pytest.raises(EngineError, match="no CPU path"):
+        Muon([p]).step()
+
+
+@pytest.mark.gpu
+def test_ortho_python_refusals_on_the_gpu():
+    from alphazero_amd import ops
+    from alphazero_amd.engine import EngineError
+
+    m = torch.zeros(3, 4, device="cuda")
+    for bad in (lambda: ops.orthogonalize([m, m.half()]), lambda: ops.orthogonalize([m, m.cpu()]), lambda: ops.orthogonalize([m[0]]),
+                lambda: ops.orthogonalize(m, coefficients=(3.0, 0.0, 0.0)), lambda: ops.orthogonalize(m, eps=-1.0), lambda: ops.orthogonalize(m, steps=2.5)):
+        with pytest.raises(EngineError):
+            bad()
