@@ -22,12 +22,14 @@ struct Args {
   const void *x, *r, *dy, *w, *b;
   void *y, *dx, *dr, *dw, *db;
   double *stats;   // [n][g]: mean, rstd
-  double *part;    // forward: [n][chunk][g] sum, sum of squares
-  float *cpart;    // backward: [n][chunk][c] sum dz, sum dz xhat
-  double *wpart;   // backward: [split][c] the same, over samples and chunks
-  int n, hw, c, g, cg, chunks, per_chunk, act, param_f32, splits;
-  float eps;
-  int64_t rows;    // n * chunks
+  double *part;    // forward, a sample in chunks: [n][chunk][g] sum, sum of squares
+  float *cpart;    // backward, a sample in chunks: [n][chunk][c] sum dz, sum dz xhat
+  float *csum;     // backward: [n][c] the same over the sample
+  float *gsum;     // backward, a sample in chunks: [n][g] mean of dz w, mean of dz w xhat
+  double *wpart;   // backward: [split][c] the channel sums of a share of the samples
+  int64_t n;
+  int hw, c, g, cg, chunks, per_chunk, act, param_f32, splits, cols, slices;
+  double eps;
 };
 
 template <class T, int V> struct alignas(sizeof(T) * V) Vec { T v[V]; };
@@ -60,21 +62,50 @@ __device__ __forceinline__ Stat stat_of(double mean, double rstd) {
 }
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + expf(-z)); }
-__device__ __forceinline__ float act_fwd(float z, int act) { return act == AZ_ACT_RELU ? (z > 0.0f || z != z ? z : 0.0f) : act == AZ_ACT_SILU ? z * sigmoid(z) : z; }
 
-// dy act'(z).  z next to 0 (closer than f32 resolves z's terms) under relu: the sign from f64
-__device__ __forceinline__ float act_bwd(float dy, float z, float x, float xh, float w, float b, float r, int act, const double *st) {
+// the activation of V values; `act` is uniform, so this is one branch for all of them
+template <int V> __device__ __forceinline__ void act_fwd(float *z, int act) {
   if (act == AZ_ACT_RELU) {
-    bool on = z > 0.0f;
-    if (__builtin_expect(fabsf(z) <= 0x1p-18f * (fabsf(xh * w) + fabsf(b) + fabsf(r)), 0))
-      on = fma(((double)x - st[0]) * st[1], (double)w, (double)b) + (double)r > 0.0;
-    return on ? dy : 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z[j] = z[j] > 0.0f || z[j] != z[j] ? z[j] : 0.0f;
+  } else if (act == AZ_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) z[j] *= sigmoid(z[j]);
   }
-  if (act == AZ_ACT_SILU) {
-    const float s = sigmoid(z);
-    return dy * (s * fmaf(z, 1.0f - s, 1.0f));
+}
+
+// V elements of a channel block: x, dy (and r) -> xhat and dz = dy act'(z).  z next to 0 (closer than f32 resolves z's terms) under
+// relu: the sign from f64
+template <int V, bool RES> __device__ __forceinline__ void grad(const float *x, const float *r, const float *w, const float *b, const Stat &st,
+                                                                const double *sd, int act, float *d, float *xh) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) xh[j] = ((x[j] - st.mh) - st.ml) * st.rs;
+  if (act == AZ_ACT_RELU) {
+    float z[V];
+    bool unsure = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float t = xh[j] * w[j], rj = RES ? r[j] : 0.0f;
+      z[j] = (t + b[j]) + rj;
+      unsure |= fabsf(z[j]) <= 0x1p-18f * (fabsf(t) + fabsf(b[j]) + fabsf(rj));
+    }
+    if (__builtin_expect(unsure, 0)) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float wj = w[j], bj = b[j];
+        asm volatile("" : "+v"(wj), "+v"(bj));  // (widened here, not ahead of the branch for every element)
+        z[j] = fma(((double)x[j] - sd[0]) * sd[1], (double)wj, (double)bj) + (double)(RES ? r[j] : 0.0f) > 0.0 ? 1.0f : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = z[j] > 0.0f ? d[j] : 0.0f;
+  } else if (act == AZ_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = fmaf(xh[j], w[j], b[j]) + (RES ? r[j] : 0.0f), s = sigmoid(z);
+      d[j] *= s * fmaf(z, 1.0f - s, 1.0f);
+    }
   }
-  return dy;
 }
 
 // How a workgroup walks pixels [p0, p1) of a sample: a pixel is CV = C / V vectors, TX threads side by side take them (looping when
@@ -127,26 +158,35 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_stats(Args 
   }
 }
 
+// mean and 1 / sqrt(var + eps) of m values with sum s and sum of squares q
+__device__ __forceinline__ void finish(double s, double q, double m, double eps, double &mean, double &rstd) {
+  mean = s / m;
+  // a group that holds an infinity or a NaN has no variance (fmax would hide it)
+  rstd = q < 1e300 ? 1.0 / sqrt(fmax(q / m - mean * mean, 0.0) + eps) : NAN;
+}
+
+// the chunks' sums -> the statistics: one wave a (sample, group)
+__global__ __launch_bounds__(NT) void k_gn_stats_join(Args a) {
+  const int64_t ng = blockIdx.x * (int64_t)(NT / 64) + (threadIdx.x >> 6), n = ng / a.g;
+  const int g = (int)(ng - n * a.g), lane = threadIdx.x & 63;
+  if (n >= a.n) return;
+  double s = 0.0, q = 0.0;
+  for (int i = lane; i < a.chunks; i += 64) { const double *p = a.part + ((n * a.chunks + i) * a.g + g) * 2; s += p[0]; q += p[1]; }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
+  if (lane == 0) finish(s, q, (double)a.hw * a.cg, a.eps, a.stats[ng * 2], a.stats[ng * 2 + 1]);
+}
+
 template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_apply(Args a) {
-  __shared__ Stat st[MAX_G];
-  const int chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
+  const int chunk = blockIdx.x % a.chunks;
   const int64_t n = blockIdx.x / a.chunks;
-  const double m = (double)a.hw * a.cg;
-  for (int g = tid; g < a.g; g += NT) {
-    double s = 0.0, q = 0.0;
-    for (int i = 0; i < a.chunks; ++i) { const double *p = a.part + ((n * a.chunks + i) * a.g + g) * 2; s += p[0]; q += p[1]; }
-    const double mean = s / m, var = fmax(q / m - mean * mean, 0.0), rstd = 1.0 / sqrt(var + (double)a.eps);
-    const double rs = q < 1e300 ? rstd : NAN;  // a sample that holds an infinity or a NaN has no variance (fmax would hide it)
-    st[g] = stat_of(mean, rs);
-    if (chunk == 0) { a.stats[(n * a.g + g) * 2] = mean; a.stats[(n * a.g + g) * 2 + 1] = rs; }
-  }
-  __syncthreads();
   const Walk k(a.c, V);
   const int p0 = chunk * a.per_chunk, p1 = min(p0 + a.per_chunk, a.hw);
   if (k.ty >= k.ty_n) return;
   const int64_t base = n * a.hw * a.c;
   for (int col = k.tx; col < k.cv; col += k.tx_n) {
-    const Stat s = st[col * V / a.cg];
+    const double *sd = a.stats + (n * a.g + col * V / a.cg) * 2;
+    const Stat s = stat_of(sd[0], sd[1]);
     float w[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
@@ -156,7 +196,8 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_apply(Args 
       load<T, V>(v, (const T *)a.x + at);
       if (a.r) load<T, V>(r, (const T *)a.r + at);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = act_fwd(fmaf(((v[j] - s.mh) - s.ml) * s.rs, w[j], b[j]) + r[j], a.act);
+      for (int j = 0; j < V; ++j) v[j] = fmaf(((v[j] - s.mh) - s.ml) * s.rs, w[j], b[j]) + r[j];
+      act_fwd<V>(v, a.act);
       store<T, V>((T *)a.y + at, v);
     }
   }
@@ -184,12 +225,12 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_sums(Ar
         load<T, V>(x, (const T *)a.x + at);
         load<T, V>(d, (const T *)a.dy + at);
         if (a.r) load<T, V>(r, (const T *)a.r + at);
+        float xh[V];
+        grad<V, true>(x, r, w, b, st, sd2, a.act, d, xh);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float xh = ((x[j] - st.mh) - st.ml) * st.rs;
-          const float dz = act_bwd(d[j], fmaf(xh, w[j], b[j]) + r[j], x[j], xh, w[j], b[j], r[j], a.act, sd2);
-          s[j] += dz;
-          q[j] = fmaf(dz, xh, q[j]);
+          s[j] += d[j];
+          q[j] = fmaf(d[j], xh[j], q[j]);
         }
       }
     }
@@ -208,21 +249,45 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_sums(Ar
   }
 }
 
-template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args a) {
-  __shared__ float c1[MAX_G], c2[MAX_G];
-  const int chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
-  const int64_t n = blockIdx.x / a.chunks, base = n * a.hw * a.c;
-  const double m = (double)a.hw * a.cg;
-  for (int g = tid; g < a.g; g += NT) {
+// the chunks' channel sums -> the sample's, and the two means a group's dx needs: one workgroup a (sample, group)
+template <class T> __global__ __launch_bounds__(NT) void k_gn_bwd_join(Args a) {
+  __shared__ double s_[NT], q_[NT], gs[NT / 64], gq[NT / 64];
+  const int64_t n = blockIdx.x / a.g;
+  const int g = (int)(blockIdx.x - n * a.g), tid = threadIdx.x;
+  const int tx_n = a.cg < NT ? a.cg : NT, ty_n = NT / tx_n, tx = tid % tx_n, ty = tid / tx_n;
+  double s1 = 0.0, q1 = 0.0;  // this thread's share of the group's weighted sums
+  for (int c0 = 0; c0 < a.cg; c0 += tx_n) {
+    const int c = g * a.cg + c0 + tx;
     double s = 0.0, q = 0.0;
-    for (int c = g * a.cg; c < (g + 1) * a.cg; ++c) {
+    if (c0 + tx < a.cg && ty < ty_n)
+      for (int i = ty; i < a.chunks; i += ty_n) { const float *p = a.cpart + ((n * a.chunks + i) * a.c + c) * 2; s += p[0]; q += p[1]; }
+    s_[tid] = s;
+    q_[tid] = q;
+    __syncthreads();
+    if (ty == 0 && c0 + tx < a.cg) {
+      for (int y = 1; y < ty_n; ++y) { s += s_[y * tx_n + tx]; q += q_[y * tx_n + tx]; }
+      a.csum[(n * a.c + c) * 2] = (float)s;
+      a.csum[(n * a.c + c) * 2 + 1] = (float)q;
       const double w = param<T>(a.w, a.param_f32, c, 1.0f);
-      for (int i = 0; i < a.chunks; ++i) { const float *p = a.cpart + ((n * a.chunks + i) * a.c + c) * 2; s = fma(w, (double)p[0], s); q = fma(w, (double)p[1], q); }
+      s1 = fma(w, s, s1);
+      q1 = fma(w, q, q1);
     }
-    c1[g] = (float)(s / m);
-    c2[g] = (float)(q / m);
+    __syncthreads();
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o); q1 += __shfl_xor(q1, o); }
+  if ((tid & 63) == 0) { gs[tid >> 6] = s1; gq[tid >> 6] = q1; }
   __syncthreads();
+  if (tid == 0) {
+    const double m = (double)a.hw * a.cg;
+    a.gsum[(n * a.g + g) * 2] = (float)((((gs[0] + gs[1]) + gs[2]) + gs[3]) / m);
+    a.gsum[(n * a.g + g) * 2 + 1] = (float)((((gq[0] + gq[1]) + gq[2]) + gq[3]) / m);
+  }
+}
+
+template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args a) {
+  const int chunk = blockIdx.x % a.chunks;
+  const int64_t n = blockIdx.x / a.chunks, base = n * a.hw * a.c;
   const Walk k(a.c, V);
   const int p0 = chunk * a.per_chunk, p1 = min(p0 + a.per_chunk, a.hw);
   if (k.ty >= k.ty_n) return;
@@ -231,7 +296,7 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args
     const double *sd = a.stats + (n * a.g + g) * 2;
     const double sd2[2] = {sd[0], sd[1]};
     const Stat st = stat_of(sd2[0], sd2[1]);
-    const float m1 = c1[g], m2 = c2[g];
+    const float m1 = a.gsum[(n * a.g + g) * 2], m2 = a.gsum[(n * a.g + g) * 2 + 1];
     float w[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
@@ -241,43 +306,207 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args
       load<T, V>(x, (const T *)a.x + at);
       load<T, V>(d, (const T *)a.dy + at);
       if (a.r) load<T, V>(r, (const T *)a.r + at);
+      float xh[V];
+      grad<V, true>(x, r, w, b, st, sd2, a.act, d, xh);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xh = ((x[j] - st.mh) - st.ml) * st.rs;
-        d[j] = act_bwd(d[j], fmaf(xh, w[j], b[j]) + r[j], x[j], xh, w[j], b[j], r[j], a.act, sd2);
-        x[j] = st.rs * (fmaf(d[j], w[j], -m1) - xh * m2);
-      }
+      for (int j = 0; j < V; ++j) x[j] = st.rs * (fmaf(d[j], w[j], -m1) - xh[j] * m2);
       if (a.dx) store<T, V>((T *)a.dx + at, x);
       if (a.dr) store<T, V>((T *)a.dr + at, d);
     }
   }
 }
 
-// per-channel sums over samples and chunks: 64 channels x 4 row lanes a workgroup, `splits` shares of the rows, then one pass over those
-template <class T> __global__ __launch_bounds__(NT) void k_gn_wb_part(Args a) {
-  __shared__ double s_[NT], q_[NT];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
-  const int64_t per = (a.rows + a.splits - 1) / a.splits, r0 = blockIdx.y * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
+// A sample's channels fit a workgroup's registers: one workgroup takes `cols` vectors (whole groups, 64 lanes at most) of every pixel
+// of a sample, so x is read once.  Its lanes keep their column for all pixels: weights, statistics and channel sums stay in registers.
+// `cols` and the vectors of a group are powers of two: lanes of one group differ in the bits below `cgv` and from `cols` on.
+template <class T> __device__ __forceinline__ void unpack(const u32x4 &w, float *o) {
+  constexpr int N = Word<T>::N;
+#pragma unroll
+  for (int j = 0; j < 4 * N; ++j) o[j] = Word<T>::get(w[j / N], j % N);
+}
+template <class T> __device__ __forceinline__ u32x4 pack(const float *o) {
+  constexpr int N = Word<T>::N;
+  return u32x4{Word<T>::put(o), Word<T>::put(o + N), Word<T>::put(o + 2 * N), Word<T>::put(o + 3 * N)};
+}
+
+// the packed words are what lives from the first use to the second: without this the compiler keeps the unpacked values too (240
+// registers instead of 100)
+__device__ __forceinline__ void packed_only(u32x4 &w) { asm volatile("" : "+v"(w)); }
+
+template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_fwd_one(Args a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ double part[NT / 64][64][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cols = a.cols, cgv = a.cg / V;
+  const int64_t n = blockIdx.x / a.slices;
+  const int col = (int)(blockIdx.x - n * a.slices) * cols + (tid & (cols - 1)), cv = a.c / V, p0 = tid / cols, step = NT / cols;
+  // the sample's bytes: a uniform base and a 32-bit offset (a resident sample has at most 4,096 pixels of 32 KiB).  Pixels behind the
+  // sample read its last one; their words are cleared before they count
+  const int64_t base = n * a.hw * a.c * (int64_t)sizeof(T);
+  const char *x = (const char *)a.x + base, *r = (const char *)a.r + base;
+  auto at = [&](int i) { return (uint32_t)(min(p0 + i * step, a.hw - 1) * cv + col) * 16u; };
+  u32x4 v[NV], rv[RES ? NV : 1];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = *(const u32x4 *)(x + at(i));
+  if (RES) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) rv[i] = *(const u32x4 *)(r + at(i));
+  }
   double s = 0.0, q = 0.0;
-  if (c < a.c)
-    for (int64_t r = r0 + lane; r < r1; r += 4) { const float *p = a.cpart + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (p0 + i * step >= a.hw) v[i] = u32x4{};
+    float f[V];
+    unpack<T>(v[i], f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) { const double d = f[j]; s += d; q = fma(d, d, q); }
+    packed_only(v[i]);
+  }
+  for (int o = 1; o < 64; o <<= 1)
+    if (o < cgv || o >= cols) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
+  const int gl = (tid & (cols - 1)) / cgv;
+  if ((lane & (cgv - 1)) == 0 && lane < cols) { part[wave][gl][0] = s; part[wave][gl][1] = q; }
+  float w[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+  __syncthreads();
+  s = ((part[0][gl][0] + part[1][gl][0]) + part[2][gl][0]) + part[3][gl][0];
+  q = ((part[0][gl][1] + part[1][gl][1]) + part[2][gl][1]) + part[3][gl][1];
+  double mean, rstd;
+  finish(s, q, (double)a.hw * a.cg, a.eps, mean, rstd);
+  const int g = col / cgv;
+  if (tid < cols && (tid & (cgv - 1)) == 0) { a.stats[(n * a.g + g) * 2] = mean; a.stats[(n * a.g + g) * 2 + 1] = rstd; }
+  const Stat st = stat_of(mean, rstd);
+  char *y = (char *)a.y + base;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float f[V], rf[V];
+    unpack<T>(v[i], f);
+    if (RES) unpack<T>(rv[i], rf);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      f[j] = fmaf(((f[j] - st.mh) - st.ml) * st.rs, w[j], b[j]);
+      if (RES) f[j] += rf[j];
+    }
+    act_fwd<V>(f, a.act);
+    const u32x4 o = pack<T>(f);
+    if (p0 + i * step < a.hw) *(u32x4 *)(y + at(i)) = o;
+  }
+}
+
+// the same for the gradient: x and dy are read once.  relu's dz is dy or 0, so it takes dy's place in its own type; silu's is computed
+// again for dx (its residual, if any, is then read again).
+template <class T, int NV, bool RES, int ACT> __global__ __launch_bounds__(NT) void k_gn_bwd_one(Args a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float part[NT / 64][64 * V][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cols = a.cols, cgv = a.cg / V;
+  const int64_t n = blockIdx.x / a.slices;
+  const int lc = tid & (cols - 1), col = (int)(blockIdx.x - n * a.slices) * cols + lc, cv = a.c / V, p0 = tid / cols, step = NT / cols;
+  const int64_t base = n * a.hw * a.c * (int64_t)sizeof(T);
+  const char *x = (const char *)a.x + base, *r = (const char *)a.r + base, *dy = (const char *)a.dy + base;
+  auto at = [&](int i) { return (uint32_t)(min(p0 + i * step, a.hw - 1) * cv + col) * 16u; };
+  u32x4 xv[NV], dv[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    xv[i] = *(const u32x4 *)(x + at(i));
+    dv[i] = *(const u32x4 *)(dy + at(i));
+  }
+  const int g = col / cgv;
+  const double sd[2] = {a.stats[(n * a.g + g) * 2], a.stats[(n * a.g + g) * 2 + 1]};
+  const Stat st = stat_of(sd[0], sd[1]);
+  float w[V], b[V], s[V] = {}, q[V] = {};
+#pragma unroll
+  for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const bool in = p0 + i * step < a.hw;
+    float xf[V], rf[V], d[V], xh[V];
+    if (RES) unpack<T>(*(const u32x4 *)(r + at(i)), rf);
+    if (!in) dv[i] = u32x4{};
+    unpack<T>(xv[i], xf);
+    unpack<T>(dv[i], d);
+    grad<V, RES>(xf, rf, w, b, st, sd, ACT, d, xh);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s[j] += d[j];
+      q[j] = fmaf(d[j], xh[j], q[j]);
+      asm volatile("" : "+v"(s[j]), "+v"(q[j]));  // (or the sums are put off until the last vector, and every d and xhat is kept)
+    }
+    if (ACT == AZ_ACT_RELU) dv[i] = pack<T>(d);  // (exact)
+    packed_only(xv[i]);
+    packed_only(dv[i]);
+  }
+  for (int o = cols; o < 64; o <<= 1) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) { s[j] += __shfl_xor(s[j], o); q[j] += __shfl_xor(q[j], o); }
+  }
+  if (lane < cols) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) { part[wave][lc * V + j][0] = s[j]; part[wave][lc * V + j][1] = q[j]; }
+  }
+  __syncthreads();
+  float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int e = lc * V + j;
+    s[j] = ((part[0][e][0] + part[1][e][0]) + part[2][e][0]) + part[3][e][0];
+    q[j] = ((part[0][e][1] + part[1][e][1]) + part[2][e][1]) + part[3][e][1];
+    m1 = fmaf(w[j], s[j], m1);
+    m2 = fmaf(w[j], q[j], m2);
+    if (tid < cols) { a.csum[(n * a.c + col * V + j) * 2] = s[j]; a.csum[(n * a.c + col * V + j) * 2 + 1] = q[j]; }
+  }
+  if (a.dx == nullptr && a.dr == nullptr) return;
+  for (int o = 1; o < cgv; o <<= 1) { m1 += __shfl_xor(m1, o); m2 += __shfl_xor(m2, o); }
+  const float inv = 1.0f / ((float)a.hw * (float)a.cg);
+  m1 *= inv;
+  m2 *= inv;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const bool in = p0 + i * step < a.hw;
+    float xf[V], rf[V], d[V], xh[V];
+    unpack<T>(xv[i], xf);
+    unpack<T>(dv[i], d);
+    if (ACT == AZ_ACT_SILU) {
+      if (RES) unpack<T>(*(const u32x4 *)(r + at(i)), rf);
+      grad<V, RES>(xf, rf, w, b, st, sd, ACT, d, xh);
+      dv[i] = pack<T>(d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) xh[j] = ((xf[j] - st.mh) - st.ml) * st.rs;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) xf[j] = st.rs * (fmaf(d[j], w[j], -m1) - xh[j] * m2);
+    const u32x4 o = pack<T>(xf);
+    if (in && a.dx) *(u32x4 *)((char *)a.dx + base + at(i)) = o;
+    if (in && a.dr) *(u32x4 *)((char *)a.dr + base + at(i)) = dv[i];
+  }
+}
+
+// the samples' channel sums -> dweight, dbias: 16 channels x 16 samples a workgroup.  Beyond 4,096 samples in `splits` shares (LAST
+// false: into wpart), joined by a second pass.
+template <class T, bool LAST> __global__ __launch_bounds__(NT) void k_gn_wb(Args a) {
+  __shared__ double s_[NT], q_[NT];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+  const bool joined = LAST && a.splits > 1;
+  const int64_t rows = joined ? a.splits : a.n, per = LAST ? rows : (rows + a.splits - 1) / a.splits;
+  const int64_t r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
+  double s = 0.0, q = 0.0;
+  if (c < a.c) {
+    if (joined) for (int64_t r = r0 + lane; r < r1; r += 16) { const double *p = a.wpart + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
+    else for (int64_t r = r0 + lane; r < r1; r += 16) { const float *p = a.csum + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
+  }
   s_[threadIdx.x] = s;
   q_[threadIdx.x] = q;
   __syncthreads();
-  if (lane == 0 && c < a.c) {
-    for (int l = 1; l < 4; ++l) { s += s_[l * 64 + threadIdx.x]; q += q_[l * 64 + threadIdx.x]; }
+  if (lane != 0 || c >= a.c) return;
+  for (int l = 1; l < 16; ++l) { s += s_[l * 16 + threadIdx.x]; q += q_[l * 16 + threadIdx.x]; }
+  if (LAST) {
+    put_param<T>(a.db, a.param_f32, c, s);
+    put_param<T>(a.dw, a.param_f32, c, q);
+  } else {
     double *o = a.wpart + ((int64_t)blockIdx.y * a.c + c) * 2;
     o[0] = s;
     o[1] = q;
   }
-}
-template <class T> __global__ __launch_bounds__(NT) void k_gn_wb(Args a) {
-  const int c = blockIdx.x * NT + threadIdx.x;
-  if (c >= a.c) return;
-  double s = 0.0, q = 0.0;
-  for (int i = 0; i < a.splits; ++i) { const double *p = a.wpart + ((int64_t)i * a.c + c) * 2; s += p[0]; q += p[1]; }
-  put_param<T>(a.db, a.param_f32, c, s);
-  put_param<T>(a.dw, a.param_f32, c, q);
 }
 
 // pixels of a sample are shared out so that there are workgroups enough, but never fewer than 32 pixels to one
@@ -285,12 +514,13 @@ static int chunks_of(int64_t n, int hw) {
   int64_t want = (2048 + n - 1) / n, most = (hw + 31) / 32;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
-static int splits_of(int64_t rows) { return rows < 256 ? 1 : rows < 16384 ? (int)(rows / 256) + 1 : 64; }
+static int splits_of(int64_t n) { return n <= 4096 ? 1 : n < 65536 ? (int)(n / 1024) : 64; }
 
+// doubles and floats of the workspace in this order: part | cpart, csum, gsum, wpart
 static int64_t ws_forward(int64_t n, int hw, int g) { return n * chunks_of(n, hw) * g * 16; }
-static int64_t ws_backward(int64_t n, int hw, int c) {
-  const int64_t rows = n * chunks_of(n, hw);
-  return rows * c * 8 + (int64_t)splits_of(rows) * c * 16;
+static int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+static int64_t ws_backward(int64_t n, int hw, int c, int g) {
+  return up16(n * chunks_of(n, hw) * c * 8) + up16(n * c * 8) + up16(n * g * 8) + (int64_t)splits_of(n) * c * 16;
 }
 
 static int check(const char *&msg, int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t g, int32_t act, double eps) {
@@ -298,7 +528,7 @@ static int check(const char *&msg, int32_t dtype, int32_t param_dtype, int64_t n
   if (param_dtype != AZ_NN_F32 && param_dtype != dtype) { msg = "group norm: weight and bias are f32 or of x's dtype"; return AZ_EINVAL; }
   if (act != AZ_ACT_NONE && act != AZ_ACT_RELU && act != AZ_ACT_SILU) { msg = "group norm: unknown activation"; return AZ_EINVAL; }
   if (n < 0 || hw < 0 || c < 1 || c > MAX_C || g < 1 || g > MAX_G || c % g) { msg = "group norm: 1 <= C <= 16,384 a multiple of the groups, at most 1,024 groups"; return AZ_EINVAL; }
-  if (n > (1 << 28) || hw > (1 << 28)) { msg = "group norm: at most 2^28 samples of 2^28 pixels"; return AZ_EINVAL; }
+  if (n > (1 << 28) || hw > (1 << 28) || n * g > 0x7FFFFFFF) { msg = "group norm: at most 2^28 samples of 2^28 pixels, 2^31 - 1 groups in all"; return AZ_EINVAL; }
   if (!(eps >= 0.0)) { msg = "group norm: eps >= 0"; return AZ_EINVAL; }
   return AZ_OK;
 }
@@ -322,6 +552,46 @@ static int vec_of(int32_t dtype, int cg, const void *const *ptrs, int np) {
   return v;
 }
 
+static int count_of(int need) { return need <= 4 ? need : need <= 6 ? 6 : need <= 8 ? 8 : need <= 12 ? 12 : 16; }  // (the vectors a thread holds)
+
+// Columns of 16 bytes a workgroup takes where a sample's share fits its registers (nv vectors a thread), or 0: whole groups, a power
+// of two, at least 64 bytes of a pixel side by side where the sample has them, and the fewest threads left idle.
+static int cols_of(int32_t dtype, int v, int c, int cg, int hw, int max_nv, int &nv) {
+  const int full = dtype == AZ_NN_F32 ? 4 : 8, cv = c / full, cgv = cg / full;
+  if (v != full || (cgv & (cgv - 1))) return 0;
+  int best = 0;
+  double waste = 0.0;
+  for (int cols = cgv > 4 ? cgv : 4; cols <= 64 && cv % cols == 0; cols *= 2) {
+    const int need = (hw * (int64_t)cols + NT - 1) / NT <= max_nv ? (int)((hw * (int64_t)cols + NT - 1) / NT) : 0;
+    if (need == 0) break;
+    const int n = count_of(need);
+    const double w = (double)n * NT / ((double)hw * cols) * (cols * 16 < 128 ? 1.1 : 1.0);
+    if (best == 0 || w < waste) { best = cols; waste = w; nv = n; }
+  }
+  if (best == 0 && cv < 4 && (cv & (cv - 1)) == 0 && cgv <= cv) {  // (fewer than 64 bytes a pixel)
+    const int64_t need = ((int64_t)hw * cv + NT - 1) / NT;
+    if (need <= max_nv) {
+      nv = count_of((int)need);
+      best = cv;
+    }
+  }
+  return best;
+}
+
+template <class F> static int by_count(int nv, F f) {
+  switch (nv) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    case 12: return f(std::integral_constant<int, 12>{});
+    default: return f(std::integral_constant<int, 16>{});
+  }
+}
+template <class F> static int by_dtype(int32_t dtype, F f) { return dtype == AZ_NN_F32 ? f(float{}) : dtype == AZ_NN_BF16 ? f(bf16_t{}) : f(f16_t{}); }
+
 }  // namespace aznorm
 
 extern "C" {
@@ -331,7 +601,7 @@ int64_t az_group_norm_workspace(int32_t backward, int64_t n, int64_t hw, int32_t
   const char *msg = "";
   if (check(msg, AZ_NN_F32, AZ_NN_F32, n, hw, c, groups, AZ_ACT_NONE, 0.0) != AZ_OK) { fail(AZ_EINVAL, msg); return -1; }
   if (n == 0 || hw == 0) return 0;
-  return backward ? ws_backward(n, (int)hw, c) : ws_forward(n, (int)hw, groups);
+  return backward ? ws_backward(n, (int)hw, c, groups) : ws_forward(n, (int)hw, groups);
 }
 
 int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t groups, int32_t act, double eps,
@@ -344,7 +614,7 @@ int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t
   const int es = dtype == AZ_NN_F32 ? 4 : 2, ps = param_dtype == AZ_NN_F32 ? 4 : 2;
   if (!x_dev || !y_dev || !stats_dev || !workspace_dev) return fail(AZ_EINVAL, "group norm: null argument");
   if (misaligned(x_dev, es) || misaligned(residual_dev, es) || misaligned(y_dev, es) || misaligned(weight_dev, ps) || misaligned(bias_dev, ps) ||
-      misaligned(stats_dev, 8) || misaligned(workspace_dev, 8))
+      misaligned(stats_dev, 8) || misaligned(workspace_dev, 16))
     return fail(AZ_EINVAL, "group norm: misaligned pointer");
   if (workspace_bytes < ws_forward(n, (int)hw, groups)) return fail(AZ_EINVAL, "group norm: workspace below az_group_norm_workspace()");
   hipStream_t s = (hipStream_t)stream;
@@ -353,14 +623,31 @@ int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t
   Args a{};
   a.x = x_dev; a.r = residual_dev; a.w = weight_dev; a.b = bias_dev; a.y = y_dev;
   a.stats = stats_dev; a.part = (double *)workspace_dev;
-  a.n = (int)n; a.hw = (int)hw; a.c = c; a.g = groups; a.cg = c / groups; a.act = act; a.param_f32 = param_dtype == AZ_NN_F32; a.eps = (float)eps;
+  a.n = n; a.hw = (int)hw; a.c = c; a.g = groups; a.cg = c / groups; a.act = act; a.param_f32 = param_dtype == AZ_NN_F32; a.eps = eps;
   a.chunks = chunks_of(n, a.hw); a.per_chunk = (a.hw + a.chunks - 1) / a.chunks;
   const void *ptrs[] = {x_dev, residual_dev, y_dev};
-  return by_type(dtype, vec_of(dtype, a.cg, ptrs, 3), [&](auto t, auto v) {
+  const int vec = vec_of(dtype, a.cg, ptrs, 3);
+  int nv = 0;
+  a.cols = cols_of(dtype, vec, c, a.cg, a.hw, 16, nv);
+  if (a.cols && n * (c / (16 / es) / a.cols) <= 0x7FFFFFFF) {
+    a.slices = c / (16 / es) / a.cols;
+    return by_dtype(dtype, [&](auto t) {
+      return by_count(nv, [&](auto k) {
+        using T = decltype(t);
+        constexpr int NV = decltype(k)::value;
+        const dim3 grid((unsigned)(n * a.slices));
+        if (a.r) hipLaunchKernelGGL((k_gn_fwd_one<T, NV, true>), grid, dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((k_gn_fwd_one<T, NV, false>), grid, dim3(NT), 0, s, a);
+        return launched("k_gn_fwd_one");
+      });
+    });
+  }
+  return by_type(dtype, vec, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     const dim3 grid((unsigned)(n * a.chunks));
     hipLaunchKernelGGL((k_gn_stats<T, V>), grid, dim3(NT), 0, s, a);
+    hipLaunchKernelGGL(k_gn_stats_join, dim3((unsigned)((n * groups + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, s, a);
     hipLaunchKernelGGL((k_gn_apply<T, V>), grid, dim3(NT), 0, s, a);
     return launched("k_gn_forward");
   });
@@ -378,38 +665,71 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
   if (!empty && (!x_dev || !dy_dev || !stats_dev || !workspace_dev)) return fail(AZ_EINVAL, "group norm: null argument");
   if (misaligned(x_dev, es) || misaligned(residual_dev, es) || misaligned(dy_dev, es) || misaligned(dx_dev, es) || misaligned(dresidual_dev, es) ||
       misaligned(weight_dev, ps) || misaligned(bias_dev, ps) || misaligned(dweight_dev, ps) || misaligned(dbias_dev, ps) || misaligned(stats_dev, 8) ||
-      misaligned(workspace_dev, 8))
+      misaligned(workspace_dev, 16))
     return fail(AZ_EINVAL, "group norm: misaligned pointer");
-  if (!empty && workspace_bytes < ws_backward(n, (int)hw, c)) return fail(AZ_EINVAL, "group norm: workspace below az_group_norm_workspace()");
+  if (!empty && workspace_bytes < ws_backward(n, (int)hw, c, groups)) return fail(AZ_EINVAL, "group norm: workspace below az_group_norm_workspace()");
   hipStream_t s = (hipStream_t)stream;
   DeviceGuard guard(s);
   if (!guard.ok) return fail(AZ_EHIP, "group norm: cannot select the stream's device");
   Args a{};
   a.x = x_dev; a.r = residual_dev; a.w = weight_dev; a.b = bias_dev; a.dy = dy_dev; a.dx = dx_dev; a.dr = dresidual_dev; a.dw = dweight_dev; a.db = dbias_dev;
   a.stats = (double *)stats_dev;
-  a.n = (int)n; a.hw = (int)hw; a.c = c; a.g = groups; a.cg = c / groups; a.act = act; a.param_f32 = param_dtype == AZ_NN_F32;
+  a.n = n; a.hw = (int)hw; a.c = c; a.g = groups; a.cg = c / groups; a.act = act; a.param_f32 = param_dtype == AZ_NN_F32;
+  a.splits = splits_of(n);
   if (empty) {  // no samples: the parameters' gradients are zero
-    a.splits = 0;
-    return by_type(dtype, 1, [&](auto t, auto) {
-      hipLaunchKernelGGL((k_gn_wb<decltype(t)>), dim3((c + NT - 1) / NT), dim3(NT), 0, s, a);
+    a.n = 0;
+    a.splits = 1;
+    return by_dtype(dtype, [&](auto t) {
+      hipLaunchKernelGGL((k_gn_wb<decltype(t), true>), dim3((c + 15) / 16), dim3(NT), 0, s, a);
       return launched("k_gn_wb");
     });
   }
   a.chunks = chunks_of(n, a.hw); a.per_chunk = (a.hw + a.chunks - 1) / a.chunks;
-  a.rows = n * a.chunks; a.splits = splits_of(a.rows);
-  a.cpart = (float *)workspace_dev; a.wpart = (double *)((char *)workspace_dev + a.rows * c * 8);
+  char *ws = (char *)workspace_dev;
+  a.cpart = (float *)ws;
+  a.csum = (float *)(ws += up16(n * a.chunks * c * 8));
+  a.gsum = (float *)(ws += up16(n * c * 8));
+  a.wpart = (double *)(ws + up16(n * groups * 8));
+  const bool params = dweight_dev || dbias_dev;
   const void *ptrs[] = {x_dev, residual_dev, dy_dev, dx_dev, dresidual_dev};
-  return by_type(dtype, vec_of(dtype, a.cg, ptrs, 5), [&](auto t, auto v) {
+  const int vec = vec_of(dtype, a.cg, ptrs, 5);
+  int nv = 0, rc;
+  a.cols = cols_of(dtype, vec, c, a.cg, a.hw, 8, nv);
+  if (a.cols && n * (c / (16 / es) / a.cols) <= 0x7FFFFFFF) {
+    a.slices = c / (16 / es) / a.cols;
+    rc = by_dtype(dtype, [&](auto t) {
+      return by_count(nv, [&](auto k) {
+        using T = decltype(t);
+        constexpr int NV = decltype(k)::value <= 8 ? decltype(k)::value : 8;
+        const dim3 grid((unsigned)(n * a.slices));
+        auto go = [&](auto act) {
+          constexpr int ACT = decltype(act)::value;
+          if (a.r) hipLaunchKernelGGL((k_gn_bwd_one<T, NV, true, ACT>), grid, dim3(NT), 0, s, a);
+          else hipLaunchKernelGGL((k_gn_bwd_one<T, NV, false, ACT>), grid, dim3(NT), 0, s, a);
+        };
+        if (act == AZ_ACT_RELU) go(std::integral_constant<int, AZ_ACT_RELU>{});
+        else if (act == AZ_ACT_SILU) go(std::integral_constant<int, AZ_ACT_SILU>{});
+        else go(std::integral_constant<int, AZ_ACT_NONE>{});
+        return launched("k_gn_bwd_one");
+      });
+    });
+  } else {
+    rc = by_type(dtype, vec, [&](auto t, auto v) {
+      using T = decltype(t);
+      constexpr int V = decltype(v)::value;
+      const dim3 grid((unsigned)(n * a.chunks));
+      hipLaunchKernelGGL((k_gn_bwd_sums<T, V>), grid, dim3(NT), 0, s, a);
+      hipLaunchKernelGGL((k_gn_bwd_join<T>), dim3((unsigned)(n * groups)), dim3(NT), 0, s, a);
+      if (dx_dev || dresidual_dev) hipLaunchKernelGGL((k_gn_bwd_dx<T, V>), grid, dim3(NT), 0, s, a);
+      return launched("k_gn_backward");
+    });
+  }
+  if (rc != AZ_OK || !params) return rc;
+  return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = decltype(v)::value;
-    const dim3 grid((unsigned)(n * a.chunks));
-    hipLaunchKernelGGL((k_gn_bwd_sums<T, V>), grid, dim3(NT), 0, s, a);
-    if (dx_dev || dresidual_dev) hipLaunchKernelGGL((k_gn_bwd_dx<T, V>), grid, dim3(NT), 0, s, a);
-    if (dweight_dev || dbias_dev) {
-      hipLaunchKernelGGL((k_gn_wb_part<T>), dim3((c + 63) / 64, a.splits), dim3(NT), 0, s, a);
-      hipLaunchKernelGGL((k_gn_wb<T>), dim3((c + NT - 1) / NT), dim3(NT), 0, s, a);
-    }
-    return launched("k_gn_backward");
+    if (a.splits > 1) hipLaunchKernelGGL((k_gn_wb<T, false>), dim3((c + 15) / 16, a.splits), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((k_gn_wb<T, true>), dim3((c + 15) / 16), dim3(NT), 0, s, a);
+    return launched("k_gn_wb");
   });
 }
 

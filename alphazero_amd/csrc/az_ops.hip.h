@@ -56,12 +56,31 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v.b << 16); }
 __device__ __forceinline__ float to_f32(f16_t v) { return (float)v.h; }
 __device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
-__device__ __forceinline__ void from_f32(float v, bf16_t &o) {
-  uint32_t u = __float_as_uint(v);
-  u = (v != v) ? 0x7FC00000u : u + 0x7FFFu + ((u >> 16) & 1u);
-  o.b = (uint16_t)(u >> 16);
-}
+__device__ __forceinline__ void from_f32(float v, bf16_t &o) { o.b = __builtin_bit_cast(uint16_t, (__bf16)v); }
 __device__ __forceinline__ void from_f32(float v, f16_t &o) { o.h = (_Float16)v; }
+
+// one 32-bit register of a tensor as floats and back: one f32, or two 16-bit elements (they stay packed in registers)
+template <class T> struct Word;
+template <> struct Word<float> {
+  static constexpr int N = 1;
+  static __device__ __forceinline__ float get(uint32_t w, int) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t put(const float *v) { return __float_as_uint(v[0]); }
+};
+template <> struct Word<bf16_t> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ float get(uint32_t w, int i) { return __uint_as_float(i ? w & 0xFFFF0000u : w << 16); }
+  static __device__ __forceinline__ uint32_t put(const float *v) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, b2{(__bf16)v[0], (__bf16)v[1]});
+  }
+};
+template <> struct Word<f16_t> {
+  static constexpr int N = 2;
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ float get(uint32_t w, int i) { return (float)__builtin_bit_cast(h2, w)[i]; }
+  static __device__ __forceinline__ uint32_t put(const float *v) { return __builtin_bit_cast(uint32_t, h2{(_Float16)v[0], (_Float16)v[1]}); }
+};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 }  // namespace azops
 

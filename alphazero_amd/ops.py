@@ -163,8 +163,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise EngineError(f"activation: one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     if not isinstance(num_groups, int) or num_groups < 1 or c < 1 or c % num_groups or c > 16384 or num_groups > 1024:
         raise EngineError(f"{c} channels in {num_groups} groups: expected 1 .. 16,384 channels, a multiple of 1 .. 1,024 groups")
-    if n > 1 << 28 or h * w > 1 << 28:
-        raise EngineError("at most 2^28 samples of 2^28 pixels")
+    if n > 1 << 28 or h * w > 1 << 28 or n * num_groups >= 1 << 31:
+        raise EngineError("at most 2^28 samples of 2^28 pixels, 2^31 - 1 groups in all")
     if not eps >= 0.0:
         raise EngineError("eps >= 0")
     dtypes = {x.dtype, torch.float32}

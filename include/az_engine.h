@@ -472,7 +472,7 @@ int az_sample_actions(int32_t dtype, int32_t rows, int32_t n, const void *scores
  * Backward: dy_dev like x; dx_dev, dresidual_dev like x, dweight_dev, dbias_dev (c) of param_dtype, each may be NULL (not wanted).
  *   relu's derivative at 0 is 0.  n * hw = 0: nothing is written but zero dweight / dbias.
  * workspace_dev: az_group_norm_workspace() bytes (backward 0 / 1; -1: refused), aligned to 16 bytes, meaningless between calls; calls that
- * overlap in time need one each.  c at most 16,384, at most 1,024 groups, 2^28 samples, 2^28 pixels.  No output may overlap an input
+ * overlap in time need one each.  c at most 16,384, at most 1,024 groups, 2^28 samples, 2^28 pixels, n * groups below 2^31.  No output may overlap an input
  * or another output.  The result does not depend on timing: sums are taken in a fixed order. */
 int64_t az_group_norm_workspace(int32_t backward, int64_t n, int64_t hw, int32_t c, int32_t groups);
 int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t groups, int32_t act, double eps,
