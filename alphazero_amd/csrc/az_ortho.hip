@@ -5,13 +5,18 @@
 //
 // All three are products of the form C[i][j] = sum_k P[i][k] Q[j][k] with k consecutive in both operands: A from X with itself, A^2
 // from the symmetric A with itself, B X from B and the transpose of X, which every step writes beside X.  Of the symmetric results
-// only the tiles on and above the diagonal are computed; the others are their mirror images.
+// only the tiles that touch the upper triangle are computed; the lower one is its mirror image.
 //
 // Arithmetic: f16 matrix instructions with f32 sums.  For f32 and f16 matrices an operand is a pair of f16, hi = f16(v) and
 // lo = f16(v - hi), and a product is hi hi + hi lo + lo hi: 22 bits of each factor, three matrix instructions, several times the rate
-// of the f32 ones.  For bf16 matrices hi alone holds more (11 bits) than the result will (8).  Stored values are scaled by powers of two
-// (X: 2^12, A and B: 2^9) so that lo stays clear of f16's smallest steps; the host bounds the singular values (az_orthogonalize), so
-// nothing overflows.  Buffers are zero padded to whole tiles and the padding stays zero: no product has a border case.
+// of the f32 ones.  For bf16 matrices hi alone holds more (11 bits) than the result will (8).  Stored values are scaled by powers of
+// two, as large as the host's bound on the singular values allows (az_orthogonalize: entries stay below 2^15), which keeps lo clear
+// of f16's smallest steps.  Buffers are zero padded to whole tiles and the padding stays
+// zero: no product has a border case.
+//
+// A row of an operand is a run of 128-byte units: 64 k of hi, or hi and lo of 32 k.  A stage of a product is one unit of every row of
+// the two panels, moved straight from memory to LDS (16 bytes a lane) while the stage before it is multiplied.  Unit r's 16-byte
+// pieces lie at piece ^ (r & 7), so that the 8 rows a quarter wave reads at once fall on different banks.
 #include "az_ops.hip.h"
 
 #include <cmath>
@@ -24,8 +29,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int NT = 256, MAX_M = 64, NORM_PARTS = 64, TILE = 64, KS = 32, PITCH = KS + 8;
-constexpr float SX = 4096.0f, SA = 512.0f;  // scales of the stored X and of the stored A and B
+constexpr int NT = 256, MAX_M = 64, NORM_PARTS = 256, UNIT = 128;
 
 struct Mat {
   const void *in;
@@ -33,82 +37,123 @@ struct Mat {
   uint64_t ws;  // byte offset of this matrix's buffers
   int32_t rows, cols;
 };
-struct Args {
+enum { GRAM, POLY, UPDATE, LAST, PACK, PHASES };  // (POLY has GRAM's tiles, LAST has UPDATE's)
+struct Table {  // what the first launch carries and leaves at the start of the workspace for the others
   Mat m[MAX_M];
-  char *ws;
-  int32_t count, planes, cur;
+  uint32_t start[3][MAX_M];  // first tile of each matrix: GRAM, UPDATE, PACK
+  int32_t count;
+};
+struct Args {
+  char *ws;  // Table, then the matrices' buffers
   float a, b, c;
+  float sx, sa, sb;  // powers of two: the stored X, A and B are sx, sa and sb times theirs
   double eps;
+  int32_t count, cur;
 };
 
-// one matrix's buffers in the workspace: norm parts (f64), then f16 planes (hi, lo): X [SP][LP], two X^T [LP][SP], A and B [SP][SP]
+// one matrix's buffers: norm parts (f64), X, two transposes of X, A, B.  SP, LP: the sides padded.
 struct Lay {
   int s, l, sp, lp, planes;
   bool tall;
-  __host__ __device__ Lay(int rows, int cols, int planes_) {
+  __host__ __device__ Lay(int rows, int cols, int planes_, int pad) {
     tall = rows > cols;
     s = tall ? cols : rows;
     l = tall ? rows : cols;
-    sp = (s + TILE - 1) / TILE * TILE;
-    lp = (l + TILE - 1) / TILE * TILE;
+    sp = (s + pad - 1) / pad * pad;
+    lp = (l + pad - 1) / pad * pad;
     planes = planes_;
   }
-  __host__ __device__ int64_t xn() const { return (int64_t)sp * lp; }
-  __host__ __device__ int64_t an() const { return (int64_t)sp * sp; }
+  __host__ __device__ int64_t xb() const { return (int64_t)sp * lp * 2 * planes; }  // bytes of X
+  __host__ __device__ int64_t ab() const { return (int64_t)sp * sp * 2 * planes; }
   __host__ __device__ int64_t x() const { return NORM_PARTS * 8; }
-  __host__ __device__ int64_t xt(int which) const { return x() + 2 * planes * xn() * (1 + which); }
+  __host__ __device__ int64_t xt(int which) const { return x() + xb() * (1 + which); }
   __host__ __device__ int64_t am() const { return xt(2); }
-  __host__ __device__ int64_t bm() const { return am() + 2 * planes * an(); }
-  __host__ __device__ int64_t bytes() const { return bm() + 2 * planes * an(); }
+  __host__ __device__ int64_t bm() const { return am() + ab(); }
+  __host__ __device__ int64_t bytes() const { return bm() + ab(); }
 };
 
-__device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo) {
-  hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+// element (row, k) of an operand with K columns: hi, and 32 elements behind it lo
+template <int P> __device__ __forceinline__ int64_t at(int64_t row, int k, int K) {
+  return P == 1 ? row * K + k : row * 2 * K + (k >> 5) * 64 + (k & 31);
+}
+// eight consecutive k (a multiple of eight): 16 bytes of each plane
+template <int P> __device__ __forceinline__ void put8(_Float16 *o, const float *v) {
+  half8 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { hi[e] = (_Float16)v[e]; lo[e] = (_Float16)(v[e] - (float)hi[e]); }
+  *(half8 *)o = hi;
+  if (P == 2) *(half8 *)(o + 32) = lo;
+}
+template <int P> __device__ __forceinline__ void get8(const _Float16 *o, float *v) {
+  const half8 hi = *(const half8 *)o;
+  half8 lo = {};
+  if (P == 2) lo = *(const half8 *)(o + 32);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
 }
 
-template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Args a) {
+template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char *ws) {
   __shared__ double s_[NT / 64];
-  const Mat m = a.m[blockIdx.y];
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = tid; i < (int)(sizeof(Table) / 4); i += NT) ((uint32_t *)ws)[i] = ((const uint32_t *)&t)[i];
+  const Mat m = t.m[blockIdx.y];
   const int64_t n = (int64_t)m.rows * m.cols;
+  constexpr int V = 16 / sizeof(T);
   double s = 0.0;
-  for (int64_t i = blockIdx.x * (int64_t)NT + threadIdx.x; i < n; i += (int64_t)NORM_PARTS * NT) {
+  const T *in = (const T *)m.in;
+  if (((uintptr_t)in & 15) == 0) {
+    const int64_t nv = n / V;
+#pragma unroll 4
+    for (int64_t i = blockIdx.x * (int64_t)NT + tid; i < nv; i += (int64_t)gridDim.x * NT) {
+      const u32x4 w = ((const u32x4 *)in)[i];
+#pragma unroll
+      for (int j = 0; j < V; ++j) { const double v = Word<T>::get(w[j / Word<T>::N], j % Word<T>::N); s = fma(v, v, s); }
+    }
+    in += nv * V;
+  }
+  for (int64_t i = (in - (const T *)m.in) + blockIdx.x * (int64_t)NT + tid; i < n; i += (int64_t)gridDim.x * NT) {
     const double v = to_f32(((const T *)m.in)[i]);
     s = fma(v, v, s);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) s_[threadIdx.x >> 6] = s;
+  if ((tid & 63) == 0) s_[tid >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) ((double *)(a.ws + m.ws))[blockIdx.x] = ((s_[0] + s_[1]) + s_[2]) + s_[3];
+  if (tid == 0) ((double *)(ws + m.ws))[blockIdx.x] = ((s_[0] + s_[1]) + s_[2]) + s_[3];
 }
 
-// block -> (matrix, tile of it) for a phase with tiles(lay) tiles a matrix
-template <class F> __device__ __forceinline__ int find(const Args &a, int &tile, F tiles) {
-  int m = 0;
-  for (; m < a.count - 1; ++m) {
-    const int t = tiles(Lay(a.m[m].rows, a.m[m].cols, a.planes));
-    if (tile < t) break;
-    tile -= t;
-  }
-  return m;
+// block -> (matrix, tile of it): the lanes look at one matrix's first tile each
+__device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
+  const uint32_t *start = ((const Table *)a.ws)->start[kind];
+  const int lane = threadIdx.x & 63;
+  const uint32_t mine = lane < a.count ? start[lane] : 0xFFFFFFFFu;
+  const int m = __popcll(__ballot(mine <= (uint32_t)tile)) - 1;
+  tile -= (int)__shfl(mine, m);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  return __builtin_amdgcn_readfirstlane(m);
 }
 
 // X0 and its transpose, scaled, split and zero padded: one 64 x 64 tile of X a workgroup
-template <class T> __global__ __launch_bounds__(NT) void k_os_pack(Args a) {
-  __shared__ float t_[TILE][TILE + 1];
+template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_pack(Args a, int parts) {
+  __shared__ float t_[64][65];
+  __shared__ double s_[NT / 64];
   int tile = blockIdx.x;
-  const int mi = find(a, tile, [](const Lay &y) { return (y.sp / TILE) * (y.lp / TILE); });
-  const Mat m = a.m[mi];
-  const Lay y(m.rows, m.cols, a.planes);
+  const int tid = threadIdx.x, mi = find(a, 2, tile);
+  const Mat m = ((const Table *)a.ws)->m[mi];
+  const Lay y(m.rows, m.cols, P, PADT);
   char *ws = a.ws + m.ws;
-  double sum = 0.0;
-  for (int i = 0; i < NORM_PARTS; ++i) sum += ((const double *)ws)[i];
+  double sum = tid < parts ? ((const double *)ws)[tid] : 0.0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((tid & 63) == 0) s_[tid >> 6] = sum;
+  __syncthreads();
+  sum = ((s_[0] + s_[1]) + s_[2]) + s_[3];
   const double norm = sqrt(sum) + a.eps;
-  const double scale = norm < 1e300 ? (norm > 0.0 ? (double)SX / norm : 0.0) : NAN;  // (no finite norm: no result)
-  const int i0 = tile / (y.lp / TILE) * TILE, j0 = tile % (y.lp / TILE) * TILE, tid = threadIdx.x;
-  for (int e = tid; e < TILE * TILE; e += NT) {
-    const int p = e / TILE, q = e % TILE;  // q runs along M's rows
+  const double scale = norm < 1e300 ? (norm > 0.0 ? (double)a.sx / norm : 0.0) : NAN;  // (no finite norm: no result)
+  const int i0 = tile / (y.lp / 64) * 64, j0 = tile % (y.lp / 64) * 64;
+  for (int e = tid; e < 64 * 64; e += NT) {
+    const int p = e / 64, q = e % 64;  // q runs along M's rows
     const int r = y.tall ? j0 + p : i0 + p, c = y.tall ? i0 + q : j0 + q;
     float v = 0.0f;
     if (r < m.rows && c < m.cols) v = (float)((double)to_f32(((const T *)m.in)[(int64_t)r * m.cols + c]) * scale);
@@ -117,124 +162,187 @@ template <class T> __global__ __launch_bounds__(NT) void k_os_pack(Args a) {
   }
   __syncthreads();
   _Float16 *x = (_Float16 *)(ws + y.x()), *xt = (_Float16 *)(ws + y.xt(0));
-  for (int e = tid; e < TILE * TILE; e += NT) {
-    const int p = e / TILE, q = e % TILE;
-    _Float16 hi, lo;
-    split(t_[p][q], hi, lo);
-    x[(int64_t)(i0 + p) * y.lp + j0 + q] = hi;
-    if (a.planes == 2) x[y.xn() + (int64_t)(i0 + p) * y.lp + j0 + q] = lo;
-    split(t_[q][p], hi, lo);
-    xt[(int64_t)(j0 + p) * y.sp + i0 + q] = hi;
-    if (a.planes == 2) xt[y.xn() + (int64_t)(j0 + p) * y.sp + i0 + q] = lo;
+  for (int e = tid; e < 64 * 8; e += NT) {
+    const int p = e / 8, q = e % 8 * 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t_[p][q + k];
+    put8<P>(x + at<P>(i0 + p, j0 + q, y.lp), v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t_[q + k][p];
+    put8<P>(xt + at<P>(j0 + p, i0 + q, y.sp), v);
   }
 }
 
-enum { GRAM, POLY, UPDATE, LAST };
+// 1 KiB from memory to LDS: 16 bytes a lane, at lds + 16 lane
+__device__ __forceinline__ void to_lds(const char *base, uint32_t lane_off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory");
+}
+// all but the newest N of this wave's moves have landed and its LDS reads are done, then the workgroup goes on
+template <int N> __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
 
-template <int PHASE> __host__ __device__ __forceinline__ int tiles_of(const Lay &y) {
-  const int s = y.sp / TILE, l = y.lp / TILE;
+// the wave's LDS writes are seen by its other lanes
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// row ti of the upper triangle of an n x n grid of tiles holds tj = ti .. n - 1
+__device__ __forceinline__ void upper(int tile, int n, int &ti, int &tj) {
+  // the row starts at ti n - ti (ti - 1) / 2
+  ti = (int)(((float)(2 * n + 1) - sqrtf((float)(2 * n + 1) * (float)(2 * n + 1) - 8.0f * (float)tile)) * 0.5f);
+  ti = ti < 0 ? 0 : ti > n - 1 ? n - 1 : ti;
+  while (ti > 0 && ti * n - ti * (ti - 1) / 2 > tile) --ti;
+  while (ti < n - 1 && (ti + 1) * n - (ti + 1) * ti / 2 <= tile) ++ti;
+  tj = ti + tile - (ti * n - ti * (ti - 1) / 2);
+}
+
+template <int PHASE> __host__ __device__ __forceinline__ int tiles_of(const Lay &y, int t) {
+  const int s = y.sp / t, l = y.lp / t;
   return PHASE == GRAM || PHASE == POLY ? s * (s + 1) / 2 : s * l;
 }
 
-template <int PHASE, int P, class T> __global__ __launch_bounds__(NT) void k_os_gemm(Args a) {
-  __shared__ __attribute__((aligned(16))) _Float16 sp_[P][TILE][PITCH], sq_[P][TILE][PITCH];
+// One T x T tile, four waves, (T / 2) x (T / 2) each in blocks of 32 x 32.  T = 64: four stages in LDS, so that the moves of three are
+// under way while one is multiplied (a launch has few such workgroups, and a stage's latency is many times its products' time);
+// T = 128: two stages, and two workgroups a CU cover for each other.
+template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) void k_os_gemm(Args a) {
+  constexpr bool SYM = PHASE == GRAM || PHASE == POLY;
+  constexpr int B = T / 64, W = T / 2, STAGE = 2 * T * UNIT, BUFS = T == 64 ? 4 : 2, MOVES = 2 * T / 8 / 4;
+  __shared__ __attribute__((aligned(1024))) char lds[BUFS * STAGE];
   int tile = blockIdx.x;
-  const int mi = find(a, tile, [](const Lay &y) { return tiles_of<PHASE>(y); });
-  const Mat m = a.m[mi];
-  const Lay y(m.rows, m.cols, P);
+  const int mi = find(a, SYM ? 0 : 1, tile);
+  const Mat m = ((const Table *)a.ws)->m[mi];
+  const Lay y(m.rows, m.cols, P, T);
   char *ws = a.ws + m.ws;
   int ti, tj;
-  if (PHASE == GRAM || PHASE == POLY) {  // row ti holds the tiles tj >= ti
-    ti = 0;
-    for (int n = y.sp / TILE; tile >= n - ti; ++ti) tile -= n - ti;
-    tj = ti + tile;
-  } else {
-    ti = tile % (y.sp / TILE);
-    tj = tile / (y.sp / TILE);
+  if (SYM) upper(tile, y.sp / T, ti, tj);
+  else {
+    ti = tile % (y.sp / T);
+    tj = tile / (y.sp / T);
   }
-  const int i0 = ti * TILE, j0 = tj * TILE;
-  const _Float16 *p, *q;
-  int64_t pn, qn;
-  int k_n;
-  if (PHASE == GRAM) { p = q = (const _Float16 *)(ws + y.x()); pn = qn = y.xn(); k_n = y.lp; }
-  else if (PHASE == POLY) { p = q = (const _Float16 *)(ws + y.am()); pn = qn = y.an(); k_n = y.sp; }
-  else { p = (const _Float16 *)(ws + y.bm()); pn = y.an(); q = (const _Float16 *)(ws + y.xt(a.cur)); qn = y.xn(); k_n = y.sp; }
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  const int lr = tid >> 2, lk = (tid & 3) * 8;  // what this thread stages: 8 k of one row
-  f32x16 acc = {};
-  for (int k0 = 0; k0 < k_n; k0 += KS) {
-    half8 vp[P], vq[P];
+  const int i0 = ti * T, j0 = tj * T, K = PHASE == GRAM ? y.lp : y.sp, pitch = K * 2 * P, stages = pitch / UNIT;
+  const char *p, *q;
+  if (PHASE == GRAM) p = q = ws + y.x();
+  else if (PHASE == POLY) p = q = ws + y.am();
+  else { p = ws + y.bm(); q = ws + y.xt(a.cur); }
+  p += (int64_t)i0 * pitch;
+  q += (int64_t)j0 * pitch;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+  const uint32_t lane_off = (uint32_t)((lane >> 3) * pitch + (((lane & 7) ^ (lane >> 3)) << 4));
+  auto issue = [&](int stage) {
+    const uint32_t dst = lds0 + (stage & (BUFS - 1)) * STAGE;
 #pragma unroll
-    for (int h = 0; h < P; ++h) {
-      vp[h] = *(const half8 *)(p + h * pn + (int64_t)(i0 + lr) * k_n + k0 + lk);
-      vq[h] = *(const half8 *)(q + h * qn + (int64_t)(j0 + lr) * k_n + k0 + lk);
+    for (int e = 0; e < MOVES; ++e) {
+      const int g = e * 4 + wave;  // eight rows of P's panel, or of Q's
+      const char *src = (g < T / 8 ? p + (int64_t)g * 8 * pitch : q + (int64_t)(g - T / 8) * 8 * pitch) + (int64_t)stage * UNIT;
+      to_lds(src, lane_off, dst + g * 1024);
     }
-    __syncthreads();
+  };
+  f32x16 acc[B][B] = {};
+  const int rp = (wi + (lane & 31)) * UNIT, rq = (T + wj + (lane & 31)) * UNIT, sw = lane & 7, hf = lane >> 5;
 #pragma unroll
-    for (int h = 0; h < P; ++h) {
-      *(half8 *)&sp_[h][lr][lk] = vp[h];
-      *(half8 *)&sq_[h][lr][lk] = vq[h];
-    }
-    __syncthreads();
+  for (int s = 0; s < BUFS - 1; ++s)
+    if (s < stages) issue(s);
+  for (int s = 0; s < stages; ++s) {
+    // stage s is here (younger ones may be under way), and stage s - 1 has been read by every wave: its buffer takes stage s + BUFS - 1
+    if (s + BUFS - 2 < stages) stage_barrier<(BUFS - 2) * MOVES>();
+    else stage_barrier<0>();
+    if (s + BUFS - 1 < stages) issue(s + BUFS - 1);
+    const char *base = lds + (s & (BUFS - 1)) * STAGE;
 #pragma unroll
-    for (int kk = 0; kk < KS; kk += 16) {
-      half8 fp[P], fq[P];
+    for (int kk = 0; kk < 4 / P; ++kk) {
+      half8 fp[B][P], fq[B][P];
 #pragma unroll
       for (int h = 0; h < P; ++h) {
-        fp[h] = *(const half8 *)&sp_[h][wi + (lane & 31)][kk + (lane >> 5) * 8];
-        fq[h] = *(const half8 *)&sq_[h][wj + (lane & 31)][kk + (lane >> 5) * 8];
+        const int piece = ((h * 4 + kk * 2 + hf) ^ sw) << 4;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+          fp[x][h] = *(const half8 *)(base + rp + x * 32 * UNIT + piece);
+          fq[x][h] = *(const half8 *)(base + rq + x * 32 * UNIT + piece);
+        }
       }
-      if (P == 2) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[P - 1], fq[0], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0], fq[P - 1], acc, 0, 0, 0);
-      }
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0], fq[0], acc, 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < B; ++x)
+#pragma unroll
+        for (int z = 0; z < B; ++z) {
+          if (P == 2) {
+            acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][P - 1], fq[z][0], acc[x][z], 0, 0, 0);
+            acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][0], fq[z][P - 1], acc[x][z], 0, 0, 0);
+          }
+          acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][0], fq[z][0], acc[x][z], 0, 0, 0);
+        }
     }
   }
-  // lane: column j of the tile, rows in groups of four
-  const int j = j0 + wj + (lane & 31);
+  stage_barrier<0>();
+  // The results go through LDS, 32 rows of a wave's share at a time (a wave uses its own strip only), so that memory sees whole units:
+  // first row by row, where the term a X or b A is added, then column by column for the mirror image or the transpose.
+  constexpr int SP_ = W + 1;
+  float *strip = (float *)lds + wave * 32 * SP_;
+  static_assert(4 * 32 * SP_ * 4 <= BUFS * STAGE, "the strips fit the stages' memory");
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int i = i0 + wi + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
-    if (PHASE == GRAM || PHASE == POLY) {
-      float v;
-      if (PHASE == GRAM) v = acc[e] * (SA / (SX * SX));
-      else {
-        const int64_t at = (int64_t)i * y.sp + j;
-        float av = (float)p[at];
-        if (P == 2) av += (float)p[pn + at];
-        v = fmaf(a.c / SA, acc[e], a.b * av);
-      }
-      _Float16 *o = (_Float16 *)(ws + (PHASE == GRAM ? y.am() : y.bm()));
-      _Float16 hi, lo;
-      split(v, hi, lo);
-      o[(int64_t)i * y.sp + j] = hi;
-      if (P == 2) o[y.an() + (int64_t)i * y.sp + j] = lo;
-      if (ti != tj) {
-        o[(int64_t)j * y.sp + i] = hi;
-        if (P == 2) o[y.an() + (int64_t)j * y.sp + i] = lo;
-      }
-    } else {
-      _Float16 *x = (_Float16 *)(ws + y.x());
-      const int64_t at = (int64_t)i * y.lp + j;
-      float xv = (float)x[at];
-      if (P == 2) xv += (float)x[y.xn() + at];
-      const float v = fmaf(a.a, xv, acc[e] * (1.0f / SA));
-      if (PHASE == LAST) {
-        if (i < y.s && j < y.l) from_f32(v * (1.0f / SX), ((T *)m.out)[y.tall ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j]);
+  for (int x = 0; x < B; ++x) {
+    // a lane holds column lane % 32 of a block, rows in groups of four
+#pragma unroll
+    for (int z = 0; z < B; ++z)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) strip[((e >> 2) * 8 + hf * 4 + (e & 3)) * SP_ + z * 32 + (lane & 31)] = acc[x][z][e];
+    wave_sync();
+    const int r0 = i0 + wi + x * 32, c0 = j0 + wj;
+    for (int e = lane; e < 32 * W / 8; e += 64) {
+      const int r = e / (W / 8), c = e % (W / 8) * 8;
+      float v[8], old[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = strip[r * SP_ + c + k];
+      if (PHASE == GRAM) {
+        const float f = a.sa / (a.sx * a.sx);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= f;
+        put8<P>((_Float16 *)(ws + y.am()) + at<P>(r0 + r, c0 + c, y.sp), v);
+      } else if (PHASE == POLY) {
+        get8<P>((const _Float16 *)(ws + y.am()) + at<P>(r0 + r, c0 + c, y.sp), old);
+        const float f = a.c * (a.sb / (a.sa * a.sa)), g = a.b * (a.sb / a.sa);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(f, v[k], g * old[k]);
+        put8<P>((_Float16 *)(ws + y.bm()) + at<P>(r0 + r, c0 + c, y.sp), v);
       } else {
-        _Float16 *xt = (_Float16 *)(ws + y.xt(a.cur ^ 1));
-        _Float16 hi, lo;
-        split(v, hi, lo);
-        x[at] = hi;
-        xt[(int64_t)j * y.sp + i] = hi;
-        if (P == 2) { x[y.xn() + at] = lo; xt[y.xn() + (int64_t)j * y.sp + i] = lo; }
+        _Float16 *o = (_Float16 *)(ws + y.x()) + at<P>(r0 + r, c0 + c, y.lp);
+        get8<P>(o, old);
+        const float f = 1.0f / a.sb;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(a.a, old[k], v[k] * f);
+        if (PHASE == UPDATE) put8<P>(o, v);
+      }
+      if (PHASE != GRAM || ti != tj) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) strip[r * SP_ + c + k] = v[k];
       }
     }
+    wave_sync();
+    if (PHASE == LAST) {  // rows and columns inside the matrix, in its own orientation
+      const float f = 1.0f / a.sx;
+      for (int e = lane; e < 32 * W; e += 64) {
+        const int r = y.tall ? e % 32 : e / W, c = y.tall ? e / 32 : e % W, i = r0 + r, j = c0 + c;
+        if (i < y.s && j < y.l) from_f32(strip[r * SP_ + c] * f, ((E *)m.out)[y.tall ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j]);
+      }
+    } else if (!SYM || ti != tj) {
+      _Float16 *o = (_Float16 *)(ws + (PHASE == GRAM ? y.am() : PHASE == POLY ? y.bm() : y.xt(a.cur ^ 1)));
+      for (int e = lane; e < W * 4; e += 64) {
+        const int c = e / 4, r = e % 4 * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = strip[(r + k) * SP_ + c];
+        put8<P>(o + at<P>(c0 + c, r0 + r, y.sp), v);
+      }
+    }
+    wave_sync();
   }
 }
 
 static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }
+
+// matrices whose products have tiles of 128 x 128 enough for the chip; the others take 64 x 64
+static int tile_of(int rows, int cols) { return (rows < cols ? rows : cols) >= 2048 ? 128 : 64; }
 
 static int check(const char *&msg, int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols) {
   if (dtype != AZ_NN_F32 && dtype != AZ_NN_BF16 && dtype != AZ_NN_F16) { msg = "orthogonalize: unknown dtype"; return AZ_EINVAL; }
@@ -245,40 +353,52 @@ static int check(const char *&msg, int32_t dtype, int32_t count, const int32_t *
 }
 
 // Singular values stay in [0, top]: top of step k + 1 is the largest |a s + b s^3 + c s^5| over [0, top of step k].  The stored X, A and
-// B are f16, so coefficients that let them grow without bound are refused.
-static bool bounded(int steps, double a, double b, double c) {
+// B are f16, so coefficients that let them grow without bound are refused.  -> the scales under which entries (at most the largest
+// singular value, its square, and the largest |b s^2 + c s^4|) stay below 2^15, half of f16's range
+static bool bounded(int steps, double a, double b, double c, Args &g) {
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-  double top = 1.0;
+  double top = 1.0, most = 1.0, poly = 0.0;
   for (int k = 0; k < steps; ++k) {
-    double next = 0.0, poly = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double s = top * i / 4096.0, s2 = s * s;
+    double next = 0.0;
+    for (int i = 0; i <= 512; ++i) {
+      const double s = top * i / 512.0, s2 = s * s;
       next = std::fmax(next, std::fabs(s * (a + s2 * (b + c * s2))));
       poly = std::fmax(poly, std::fabs(s2 * (b + c * s2)));
     }
     if (!(poly < 100.0) || !(next < 7.5)) return false;
     top = next * 1.001;
+    most = std::fmax(most, top);
   }
+  auto scale = [](double largest) { return (float)std::exp2(std::floor(std::log2(32768.0 / std::fmax(largest, 1.0)))); };
+  g.sx = scale(most);
+  g.sa = scale(most * most);
+  g.sb = scale(poly);
   return true;
 }
 
-template <class T, int P> static int run(const Args &base, int steps, hipStream_t s) {
-  Args a = base;
-  int t[4] = {0, 0, 0, 0}, pack = 0;
-  for (int i = 0; i < a.count; ++i) {
-    const Lay y(a.m[i].rows, a.m[i].cols, P);
-    t[GRAM] += tiles_of<GRAM>(y);
-    t[UPDATE] += tiles_of<UPDATE>(y);
-    pack += (y.sp / TILE) * (y.lp / TILE);
+// matrices of one tile size, at most MAX_M, in one run of launches
+template <class E, int P, int T> static int run(Table &t, Args a, int steps, hipStream_t s) {
+  uint32_t n[3] = {0, 0, 0};
+  int64_t most = 0;
+  for (int i = 0; i < t.count; ++i) {
+    const Lay y(t.m[i].rows, t.m[i].cols, P, T);
+    const uint32_t add[3] = {(uint32_t)tiles_of<GRAM>(y, T), (uint32_t)tiles_of<UPDATE>(y, T), (uint32_t)(y.sp / 64) * (uint32_t)(y.lp / 64)};
+    for (int k = 0; k < 3; ++k) { t.start[k][i] = n[k]; n[k] += add[k]; }
+    const int64_t e = (int64_t)t.m[i].rows * t.m[i].cols;
+    most = e > most ? e : most;
   }
-  hipLaunchKernelGGL((k_os_norm<T>), dim3(NORM_PARTS, a.count), dim3(NT), 0, s, a);
-  hipLaunchKernelGGL((k_os_pack<T>), dim3(pack), dim3(NT), 0, s, a);
+  // the norm's workgroups: 16 Ki elements each for the largest matrix
+  const int64_t want = (most + 16383) / 16384;
+  const int parts = (int)(want < 1 ? 1 : want < NORM_PARTS ? want : NORM_PARTS);
+  a.count = t.count;
+  hipLaunchKernelGGL((k_os_norm<E>), dim3(parts, t.count), dim3(NT), 0, s, t, a.ws);
+  hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(n[2]), dim3(NT), 0, s, a, parts);
   for (int k = 0; k < steps; ++k) {
     a.cur = k & 1;
-    hipLaunchKernelGGL((k_os_gemm<GRAM, P, T>), dim3(t[GRAM]), dim3(NT), 0, s, a);
-    hipLaunchKernelGGL((k_os_gemm<POLY, P, T>), dim3(t[GRAM]), dim3(NT), 0, s, a);
-    if (k + 1 < steps) hipLaunchKernelGGL((k_os_gemm<UPDATE, P, T>), dim3(t[UPDATE]), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((k_os_gemm<LAST, P, T>), dim3(t[UPDATE]), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E>), dim3(n[0]), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E>), dim3(n[0]), dim3(NT), 0, s, a);
+    if (k + 1 < steps) hipLaunchKernelGGL((k_os_gemm<UPDATE, P, T, E>), dim3(n[1]), dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((k_os_gemm<LAST, P, T, E>), dim3(n[1]), dim3(NT), 0, s, a);
   }
   return launched("k_os");
 }
@@ -293,8 +413,8 @@ int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *
   if (check(msg, dtype, count, rows, cols) != AZ_OK) { fail(AZ_EINVAL, msg); return -1; }
   int64_t total = 0;
   for (int i = 0; i < count; ++i)
-    if (rows[i] > 0 && cols[i] > 0) total += round_up(Lay(rows[i], cols[i], dtype == AZ_NN_BF16 ? 1 : 2).bytes());
-  return total;
+    if (rows[i] > 0 && cols[i] > 0) total += round_up(Lay(rows[i], cols[i], dtype == AZ_NN_BF16 ? 1 : 2, tile_of(rows[i], cols[i])).bytes());
+  return total ? total + round_up(sizeof(Table)) : 0;
 }
 
 int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols,
@@ -304,7 +424,8 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
   if (check(msg, dtype, count, rows, cols) != AZ_OK) return fail(AZ_EINVAL, msg);
   if (steps < 1 || steps > 64) return fail(AZ_EINVAL, "orthogonalize: 1 .. 64 steps");
   if (!(eps >= 0.0 && eps < 1e300)) return fail(AZ_EINVAL, "orthogonalize: eps >= 0");
-  if (!bounded(steps, a, b, c)) return fail(AZ_EINVAL, "orthogonalize: these coefficients let singular values grow beyond 7.5 (or the polynomial beyond 100)");
+  Args g{};
+  if (!bounded(steps, a, b, c, g)) return fail(AZ_EINVAL, "orthogonalize: these coefficients let singular values grow beyond 7.5 (or the polynomial beyond 100)");
   const int es = dtype == AZ_NN_F32 ? 4 : 2, planes = dtype == AZ_NN_BF16 ? 1 : 2;
   if (count > 0 && (!in || !out)) return fail(AZ_EINVAL, "orthogonalize: null argument");
   int live = 0;
@@ -319,20 +440,26 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
   hipStream_t s = (hipStream_t)stream;
   DeviceGuard guard(s);
   if (!guard.ok) return fail(AZ_EHIP, "orthogonalize: cannot select the stream's device");
-  Args g{};
   g.ws = (char *)workspace_dev;
-  g.planes = planes;
   g.a = (float)a; g.b = (float)b; g.c = (float)c; g.eps = eps;
-  uint64_t off = 0;
-  for (int i = 0; i < count; ++i) {
-    if (rows[i] == 0 || cols[i] == 0) continue;
-    g.m[g.count++] = Mat{in[i], out[i], off, rows[i], cols[i]};
-    off += (uint64_t)round_up(Lay(rows[i], cols[i], planes).bytes());
-    --live;
-    if (g.count == MAX_M || live == 0) {
-      const int rc = dtype == AZ_NN_F32 ? run<float, 2>(g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1>(g, steps, s) : run<f16_t, 2>(g, steps, s);
-      if (rc != AZ_OK) return rc;
-      g.count = 0;
+  for (int tile = 64; tile <= 128; tile *= 2) {  // (runs follow each other on the stream: they share the table, and the buffers are their own)
+    Table t;
+    t.count = 0;
+    uint64_t off = round_up(sizeof(Table));
+    for (int i = 0; i < count; ++i) {
+      const bool here = rows[i] > 0 && cols[i] > 0 && tile_of(rows[i], cols[i]) == tile;
+      if (here) {
+        t.m[t.count++] = Mat{in[i], out[i], off, rows[i], cols[i]};
+        off += (uint64_t)round_up(Lay(rows[i], cols[i], planes, tile).bytes());
+      }
+      if (t.count == MAX_M || (i == count - 1 && t.count > 0)) {
+        int rc;
+        if (tile == 64) rc = dtype == AZ_NN_F32 ? run<float, 2, 64>(t, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 64>(t, g, steps, s) : run<f16_t, 2, 64>(t, g, steps, s);
+        else rc = dtype == AZ_NN_F32 ? run<float, 2, 128>(t, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 128>(t, g, steps, s) : run<f16_t, 2, 128>(t, g, steps, s);
+        if (rc != AZ_OK) return rc;
+        t.count = 0;
+        off = round_up(sizeof(Table));
+      }
     }
   }
   return AZ_OK;
