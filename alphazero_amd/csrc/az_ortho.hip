@@ -239,7 +239,7 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
       to_lds(src, lane_off, dst + g * 1024);
     }
   };
-  f32x16 acc[B][B] = {};
+  f32x16 acc[B][B] = {}, low[P == 2 ? B : 1][P == 2 ? B : 1] = {};  // hi hi; hi lo + lo hi, joined at the end: a third of the roundings
   const int rp = (wi + (lane & 31)) * UNIT, rq = (T + wj + (lane & 31)) * UNIT, sw = lane & 7, hf = lane >> 5;
 #pragma unroll
   for (int s = 0; s < BUFS - 1; ++s)
@@ -267,8 +267,8 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
 #pragma unroll
         for (int z = 0; z < B; ++z) {
           if (P == 2) {
-            acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][P - 1], fq[z][0], acc[x][z], 0, 0, 0);
-            acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][0], fq[z][P - 1], acc[x][z], 0, 0, 0);
+            low[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][P - 1], fq[z][0], low[x][z], 0, 0, 0);
+            low[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][0], fq[z][P - 1], low[x][z], 0, 0, 0);
           }
           acc[x][z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[x][0], fq[z][0], acc[x][z], 0, 0, 0);
         }
@@ -286,7 +286,7 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
 #pragma unroll
     for (int z = 0; z < B; ++z)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) strip[((e >> 2) * 8 + hf * 4 + (e & 3)) * SP_ + z * 32 + (lane & 31)] = acc[x][z][e];
+      for (int e = 0; e < 16; ++e) strip[((e >> 2) * 8 + hf * 4 + (e & 3)) * SP_ + z * 32 + (lane & 31)] = P == 2 ? acc[x][z][e] + low[x][z][e] : acc[x][z][e];
     wave_sync();
     const int r0 = i0 + wi + x * 32, c0 = j0 + wj;
     for (int e = lane; e < 32 * W / 8; e += 64) {
