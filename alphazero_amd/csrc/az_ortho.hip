@@ -37,10 +37,12 @@ struct Mat {
   uint64_t ws;  // byte offset of this matrix's buffers
   int32_t rows, cols;
 };
-enum { GRAM, POLY, UPDATE, LAST, PACK, PHASES };  // (POLY has GRAM's tiles, LAST has UPDATE's)
+enum { GRAM, POLY, UPDATE, LAST };  // (POLY has GRAM's tiles, LAST has UPDATE's)
+enum { WHOLE, PART, JOIN };  // a tile's product at once; a share of its k range; the shares' sum and what follows a product
 struct Table {  // what the first launch carries and leaves at the start of the workspace for the others
   Mat m[MAX_M];
-  uint32_t start[3][MAX_M];  // first tile of each matrix: GRAM, UPDATE, PACK
+  uint32_t start[4][MAX_M];  // first tile of each matrix: of A and B, of X, of PACK; first partial tile of A
+  int32_t shares[MAX_M];     // of A's k range
   int32_t count;
 };
 struct Args {
@@ -49,6 +51,8 @@ struct Args {
   float sx, sa, sb;  // powers of two: the stored X, A and B are sx, sa and sb times theirs
   double eps;
   int32_t count, cur;
+  int32_t n[4];     // tiles in all, as in Table::start
+  uint64_t part;    // byte offset of the partial tiles
 };
 
 // one matrix's buffers: norm parts (f64), X, two transposes of X, A, B.  SP, LP: the sides padded.
@@ -123,7 +127,15 @@ template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char
   if (tid == 0) ((double *)(ws + m.ws))[blockIdx.x] = ((s_[0] + s_[1]) + s_[2]) + s_[3];
 }
 
-// block -> (matrix, tile of it): the lanes look at one matrix's first tile each
+// Workgroups go round the 8 XCDs in turn; block b takes item (b % 8) * ceil(n / 8) + b / 8 of n, so that an XCD (and its L2) gets a
+// run of neighbouring tiles, and much the same matrices in every phase.  -> -1: none (the grid is rounded up to whole turns)
+__device__ __forceinline__ int item_of(int n) {
+  const int per = (n + 7) / 8, t = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  return (int)(blockIdx.x >> 3) < per && t < n ? t : -1;
+}
+static unsigned grid_of(uint32_t n) { return (n + 7) / 8 * 8; }
+
+// tile -> (matrix, tile of it): the lanes look at one matrix's first tile each
 __device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
   const uint32_t *start = ((const Table *)a.ws)->start[kind];
   const int lane = threadIdx.x & 63;
@@ -138,7 +150,8 @@ __device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
 template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_pack(Args a, int parts) {
   __shared__ float t_[64][65];
   __shared__ double s_[NT / 64];
-  int tile = blockIdx.x;
+  int tile = item_of(a.n[2]);
+  if (tile < 0) return;
   const int tid = threadIdx.x, mi = find(a, 2, tile);
   const Mat m = ((const Table *)a.ws)->m[mi];
   const Lay y(m.rows, m.cols, P, PADT);
@@ -202,15 +215,22 @@ template <int PHASE> __host__ __device__ __forceinline__ int tiles_of(const Lay 
   return PHASE == GRAM || PHASE == POLY ? s * (s + 1) / 2 : s * l;
 }
 
-// One T x T tile, four waves, (T / 2) x (T / 2) each in blocks of 32 x 32.  T = 64: four stages in LDS, so that the moves of three are
-// under way while one is multiplied (a launch has few such workgroups, and a stage's latency is many times its products' time);
-// T = 128: two stages, and two workgroups a CU cover for each other.
-template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) void k_os_gemm(Args a) {
+// One T x T tile, four waves, (T / 2) x (T / 2) each in blocks of 32 x 32.  T = 64, and T = 128 with two planes, which leaves a CU one
+// workgroup: four stages in LDS, the moves of three under way while one is multiplied.  T = 128 with one plane: two stages, and two
+// workgroups a CU cover for each other.
+// A long A with few tiles is cut along k (PART): every share leaves its sums as they lie in its registers, and JOIN adds the shares in
+// order and goes on as WHOLE does.
+template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds__(NT) void k_os_gemm(Args a) {
   constexpr bool SYM = PHASE == GRAM || PHASE == POLY;
-  constexpr int B = T / 64, W = T / 2, STAGE = 2 * T * UNIT, BUFS = T == 64 ? 4 : 2, MOVES = 2 * T / 8 / 4;
+  constexpr int B = T / 64, W = T / 2, STAGE = 2 * T * UNIT, BUFS = T == 64 || P == 2 ? 4 : 2, MOVES = 2 * T / 8 / 4;
   __shared__ __attribute__((aligned(1024))) char lds[BUFS * STAGE];
-  int tile = blockIdx.x;
-  const int mi = find(a, SYM ? 0 : 1, tile);
+  constexpr int KIND = MODE == PART ? 3 : SYM ? 0 : 1;
+  int tile = item_of(a.n[KIND]);
+  if (tile < 0) return;
+  const int mi = find(a, KIND, tile);
+  const int shares = MODE == WHOLE ? 1 : ((const Table *)a.ws)->shares[mi], share = MODE == PART ? tile % shares : 0;
+  if (MODE == PART) tile /= shares;
+  const int64_t first = MODE == WHOLE ? 0 : (int64_t)((const Table *)a.ws)->start[3][mi] + (int64_t)tile * shares + share;  // partial tile
   const Mat m = ((const Table *)a.ws)->m[mi];
   const Lay y(m.rows, m.cols, P, T);
   char *ws = a.ws + m.ws;
@@ -241,14 +261,16 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
   };
   f32x16 acc[B][B] = {}, low[P == 2 ? B : 1][P == 2 ? B : 1] = {};  // hi hi; hi lo + lo hi, joined at the end: a third of the roundings
   const int rp = (wi + (lane & 31)) * UNIT, rq = (T + wj + (lane & 31)) * UNIT, sw = lane & 7, hf = lane >> 5;
+  if constexpr (MODE != JOIN) {
+  const int s0 = MODE == PART ? (int)((int64_t)stages * share / shares) : 0, s1 = MODE == PART ? (int)((int64_t)stages * (share + 1) / shares) : stages;
 #pragma unroll
   for (int s = 0; s < BUFS - 1; ++s)
-    if (s < stages) issue(s);
-  for (int s = 0; s < stages; ++s) {
+    if (s0 + s < s1) issue(s0 + s);
+  for (int s = s0; s < s1; ++s) {
     // stage s is here (younger ones may be under way), and stage s - 1 has been read by every wave: its buffer takes stage s + BUFS - 1
-    if (s + BUFS - 2 < stages) stage_barrier<(BUFS - 2) * MOVES>();
+    if (s + BUFS - 2 < s1) stage_barrier<(BUFS - 2) * MOVES>();
     else stage_barrier<0>();
-    if (s + BUFS - 1 < stages) issue(s + BUFS - 1);
+    if (s + BUFS - 1 < s1) issue(s + BUFS - 1);
     const char *base = lds + (s & (BUFS - 1)) * STAGE;
 #pragma unroll
     for (int kk = 0; kk < 4 / P; ++kk) {
@@ -275,6 +297,26 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
     }
   }
   stage_barrier<0>();
+  }
+  if constexpr (MODE != WHOLE) {
+    // [tile][share][block][element][thread] f32
+    constexpr int64_t STEP = (int64_t)B * B * 16 * NT;
+    float *part = (float *)(a.ws + a.part) + first * STEP + tid;
+    for (int k = 0; k < (MODE == PART ? 1 : shares); ++k) {
+#pragma unroll
+      for (int x = 0; x < B; ++x)
+#pragma unroll
+        for (int z = 0; z < B; ++z)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float *q_ = part + ((x * B + z) * 16 + e) * NT;
+            if (MODE == PART) *q_ = P == 2 ? acc[x][z][e] + low[x][z][e] : acc[x][z][e];
+            else acc[x][z][e] += *q_;
+          }
+      part += STEP;
+    }
+    if (MODE == PART) return;
+  }
   // The results go through LDS, 32 rows of a wave's share at a time (a wave uses its own strip only), so that memory sees whole units:
   // first row by row, where the term a X or b A is added, then column by column for the mirror image or the transpose.
   constexpr int SP_ = W + 1;
@@ -341,8 +383,18 @@ template <int PHASE, int P, int T, class E> __global__ __launch_bounds__(NT) voi
 
 static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }
 
-// matrices whose products have tiles of 128 x 128 enough for the chip; the others take 64 x 64
-static int tile_of(int rows, int cols) { return (rows < cols ? rows : cols) >= 2048 ? 128 : 64; }
+// tile side by the short side: measured on 1536 x 1536 / 2000 x 4096, 64 takes 0.47 / 1.54 ms in f32 and 0.25 / 0.76 ms in bf16, 128 takes
+// 0.53 / 1.34 and 0.34 / 0.59
+static int tile_of(int rows, int cols) { return (rows < cols ? rows : cols) >= 1792 ? 128 : 64; }
+
+// Shares of A's k range, by the matrix alone (a matrix's result must not depend on the others in the call): at most 96 tiles of 64 x 64
+// leave CUs idle, and with 32 stages or more a share of 8 stages or more is worth the second pass.
+static int shares_of(const Lay &y, int tile) {
+  const int tiles = tiles_of<GRAM>(y, tile), stages = y.lp * 2 * y.planes / UNIT;
+  if (tile != 64 || tiles > 96 || stages < 32) return 1;
+  const int s = 512 / tiles < stages / 8 ? 512 / tiles : stages / 8;
+  return s < 8 ? s : 8;
+}
 
 static int check(const char *&msg, int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols) {
   if (dtype != AZ_NN_F32 && dtype != AZ_NN_BF16 && dtype != AZ_NN_F16) { msg = "orthogonalize: unknown dtype"; return AZ_EINVAL; }
@@ -376,29 +428,79 @@ static bool bounded(int steps, double a, double b, double c, Args &g) {
   return true;
 }
 
-// matrices of one tile size, at most MAX_M, in one run of launches
-template <class E, int P, int T> static int run(Table &t, Args a, int steps, hipStream_t s) {
-  uint32_t n[3] = {0, 0, 0};
+// One run of launches: up to MAX_M matrices of one tile size, and where everything lies in the workspace.
+struct Run {
+  Table t;
+  int tile;
+  bool shared;  // some A is cut
+  uint32_t n[4];
+  uint64_t part, bytes;
+};
+
+// f(Run &) for every run of the call; in / out may be null (sizes only)
+template <class F> static int each_run(int planes, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, F f) {
+  for (int tile = 64; tile <= 128; tile *= 2) {
+    Run r;
+    r.t.count = 0;
+    for (int i = 0; i < count; ++i) {
+      if (rows[i] > 0 && cols[i] > 0 && tile_of(rows[i], cols[i]) == tile) {
+        r.t.m[r.t.count++] = Mat{in ? in[i] : nullptr, out ? out[i] : nullptr, 0, rows[i], cols[i]};
+      }
+      if (r.t.count == 0 || (r.t.count < MAX_M && i < count - 1)) continue;
+      uint64_t off = round_up(sizeof(Table));
+      r.tile = tile;
+      r.shared = false;
+      for (uint32_t &v : r.n) v = 0;
+      for (int k = 0; k < r.t.count; ++k) {
+        Mat &m = r.t.m[k];
+        const Lay y(m.rows, m.cols, planes, tile);
+        m.ws = off;
+        off += (uint64_t)round_up(y.bytes());
+        const int shares = shares_of(y, tile), sym = tiles_of<GRAM>(y, tile);
+        r.t.shares[k] = shares;
+        r.shared |= shares > 1;
+        const uint32_t add[4] = {(uint32_t)sym, (uint32_t)tiles_of<UPDATE>(y, tile), (uint32_t)(y.sp / 64) * (uint32_t)(y.lp / 64), (uint32_t)(sym * shares)};
+        for (int q = 0; q < 4; ++q) { r.t.start[q][k] = r.n[q]; r.n[q] += add[q]; }
+      }
+      r.part = off;
+      if (r.shared) off += (uint64_t)r.n[3] * tile * tile * 4;
+      r.bytes = off;
+      const int rc = f(r);
+      if (rc != AZ_OK) return rc;
+      r.t.count = 0;
+    }
+  }
+  return AZ_OK;
+}
+
+template <class E, int P, int T> static int run(const Run &r, Args a, int steps, hipStream_t s) {
   int64_t most = 0;
-  for (int i = 0; i < t.count; ++i) {
-    const Lay y(t.m[i].rows, t.m[i].cols, P, T);
-    const uint32_t add[3] = {(uint32_t)tiles_of<GRAM>(y, T), (uint32_t)tiles_of<UPDATE>(y, T), (uint32_t)(y.sp / 64) * (uint32_t)(y.lp / 64)};
-    for (int k = 0; k < 3; ++k) { t.start[k][i] = n[k]; n[k] += add[k]; }
-    const int64_t e = (int64_t)t.m[i].rows * t.m[i].cols;
+  for (int i = 0; i < r.t.count; ++i) {
+    const int64_t e = (int64_t)r.t.m[i].rows * r.t.m[i].cols;
     most = e > most ? e : most;
   }
   // the norm's workgroups: 16 Ki elements each for the largest matrix
   const int64_t want = (most + 16383) / 16384;
   const int parts = (int)(want < 1 ? 1 : want < NORM_PARTS ? want : NORM_PARTS);
-  a.count = t.count;
-  hipLaunchKernelGGL((k_os_norm<E>), dim3(parts, t.count), dim3(NT), 0, s, t, a.ws);
-  hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(n[2]), dim3(NT), 0, s, a, parts);
+  a.count = r.t.count;
+  a.part = r.part;
+  for (int k = 0; k < 4; ++k) a.n[k] = (int)r.n[k];
+  const dim3 sym(grid_of(r.n[0])), all(grid_of(r.n[1]));
+  hipLaunchKernelGGL((k_os_norm<E>), dim3(parts, r.t.count), dim3(NT), 0, s, r.t, a.ws);
+  hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(grid_of(r.n[2])), dim3(NT), 0, s, a, parts);
   for (int k = 0; k < steps; ++k) {
     a.cur = k & 1;
-    hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E>), dim3(n[0]), dim3(NT), 0, s, a);
-    hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E>), dim3(n[0]), dim3(NT), 0, s, a);
-    if (k + 1 < steps) hipLaunchKernelGGL((k_os_gemm<UPDATE, P, T, E>), dim3(n[1]), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((k_os_gemm<LAST, P, T, E>), dim3(n[1]), dim3(NT), 0, s, a);
+    if (r.shared) {
+      if constexpr (T == 64) {
+        hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, PART>), dim3(grid_of(r.n[3])), dim3(NT), 0, s, a);
+        hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, JOIN>), sym, dim3(NT), 0, s, a);
+      }
+    } else {
+      hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, WHOLE>), sym, dim3(NT), 0, s, a);
+    }
+    hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E, WHOLE>), sym, dim3(NT), 0, s, a);
+    if (k + 1 < steps) hipLaunchKernelGGL((k_os_gemm<UPDATE, P, T, E, WHOLE>), all, dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((k_os_gemm<LAST, P, T, E, WHOLE>), all, dim3(NT), 0, s, a);
   }
   return launched("k_os");
 }
@@ -411,10 +513,12 @@ int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *
   using namespace azortho;
   const char *msg = "";
   if (check(msg, dtype, count, rows, cols) != AZ_OK) { fail(AZ_EINVAL, msg); return -1; }
-  int64_t total = 0;
-  for (int i = 0; i < count; ++i)
-    if (rows[i] > 0 && cols[i] > 0) total += round_up(Lay(rows[i], cols[i], dtype == AZ_NN_BF16 ? 1 : 2, tile_of(rows[i], cols[i])).bytes());
-  return total ? total + round_up(sizeof(Table)) : 0;
+  uint64_t most = 0;  // (runs follow each other on the stream: they share the memory)
+  each_run(dtype == AZ_NN_BF16 ? 1 : 2, count, nullptr, nullptr, rows, cols, [&](const Run &r) {
+    most = r.bytes > most ? r.bytes : most;
+    return AZ_OK;
+  });
+  return (int64_t)most;
 }
 
 int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols,
@@ -442,27 +546,10 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
   if (!guard.ok) return fail(AZ_EHIP, "orthogonalize: cannot select the stream's device");
   g.ws = (char *)workspace_dev;
   g.a = (float)a; g.b = (float)b; g.c = (float)c; g.eps = eps;
-  for (int tile = 64; tile <= 128; tile *= 2) {  // (runs follow each other on the stream: they share the table, and the buffers are their own)
-    Table t;
-    t.count = 0;
-    uint64_t off = round_up(sizeof(Table));
-    for (int i = 0; i < count; ++i) {
-      const bool here = rows[i] > 0 && cols[i] > 0 && tile_of(rows[i], cols[i]) == tile;
-      if (here) {
-        t.m[t.count++] = Mat{in[i], out[i], off, rows[i], cols[i]};
-        off += (uint64_t)round_up(Lay(rows[i], cols[i], planes, tile).bytes());
-      }
-      if (t.count == MAX_M || (i == count - 1 && t.count > 0)) {
-        int rc;
-        if (tile == 64) rc = dtype == AZ_NN_F32 ? run<float, 2, 64>(t, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 64>(t, g, steps, s) : run<f16_t, 2, 64>(t, g, steps, s);
-        else rc = dtype == AZ_NN_F32 ? run<float, 2, 128>(t, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 128>(t, g, steps, s) : run<f16_t, 2, 128>(t, g, steps, s);
-        if (rc != AZ_OK) return rc;
-        t.count = 0;
-        off = round_up(sizeof(Table));
-      }
-    }
-  }
-  return AZ_OK;
+  return each_run(planes, count, in, out, rows, cols, [&](const Run &r) {
+    if (r.tile == 64) return dtype == AZ_NN_F32 ? run<float, 2, 64>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 64>(r, g, steps, s) : run<f16_t, 2, 64>(r, g, steps, s);
+    return dtype == AZ_NN_F32 ? run<float, 2, 128>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 128>(r, g, steps, s) : run<f16_t, 2, 128>(r, g, steps, s);
+  });
 }
 
 }  // extern "C"
