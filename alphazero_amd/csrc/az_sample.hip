@@ -10,8 +10,13 @@
 // rounded once, by at most 2^-45 of the largest; an f32 mass (2^-24) would move the border between neighbours of long rows.
 // At most 2^19 scores per row keep the sum below 2^63.
 //
-// The kept set is a prefix of the order, so it is described by its last member (key, index), and no row is ever sorted: the
-// prefix's end is found from histograms over the 32-bit order-preserving image of the score.
+// The kept set is a prefix of the order, so it is described by its last member (key, index), and no row is ever sorted.
+//
+//   n <= 1,024: a row is one wave's, in registers; the prefix's end is bisected over the score, counting with ballots
+//   longer:     a row is one workgroup's, which walks it a few times (after the first time it comes from the caches); the prefix's
+//               end comes from a histogram linear in the score and a list of the scores in the bin it falls into
+//
+// Bound by the exponentials: about 25 f64 operations each, at most two per score (the mass of the whole row, the kept mass).
 #include "az_ops.hip.h"
 
 namespace azsample {
@@ -19,7 +24,7 @@ namespace azsample {
 using namespace azops;
 typedef unsigned long long u64;
 
-constexpr int MAX_N = 1 << 19, BINS = 2048, NT = 256, WAVES = NT / 64;
+constexpr int MAX_N = 1 << 19, BINS = 2048, LIST = 1024;
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;  // the image of -inf: masked, NaN and -inf scores
 constexpr uint32_t KEY_PINF = 0xFF800000u;
 constexpr double UNIT = 17592186044416.0;  // 2^44
@@ -68,34 +73,257 @@ __device__ __forceinline__ u64 weight(uint32_t key, double m, double sc, bool in
   return (u64)__double_as_longlong(ldexp(r, (int)kf + 44) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// Wave reductions by data-parallel moves (rows of 16 lanes, then across rows): no LDS round trips.  The result is in lane 63 of a scan.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 moved(u64 v) {
+  return ((u64)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | moved<CTRL, ROWS>((uint32_t)v);
+}
+template <class N> __device__ __forceinline__ N wave_scan(N v) {  // inclusive sum over lanes
+  v += moved<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3
+  v += moved<0x143, 0xC>(v);  // row_bcast 31 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+  return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ u64 wave_sum(u64 v) { return lane_of(wave_scan(v), 63); }
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const uint32_t x = __shfl_xor(v, o); v = x > v ? x : v; }
-  return v;
-}
-__device__ __forceinline__ u64 wave_scan(u64 v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const u64 x = __shfl_up(v, o); v += lane >= o ? x : 0; }
-  return v;
+  auto up = [&](uint32_t x) { v = x > v ? x : v; };
+  up(moved<0x111, 0xF>(v));
+  up(moved<0x112, 0xF>(v));
+  up(moved<0x114, 0xF>(v));
+  up(moved<0x118, 0xF>(v));
+  up(moved<0x142, 0xA>(v));
+  up(moved<0x143, 0xC>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-struct Shared {
-  u64 hist[BINS];
-  u64 part[WAVES];
-  uint32_t kmax[WAVES], kmin[WAVES];
-  u64 base, value;
-  int32_t bin, tie;
+struct Setting {  // of one row
+  double sc, p, least;
+  int k;
+  float u;
 };
+__device__ __forceinline__ Setting setting_of(const Args &a, int64_t r) {
+  double t = a.t_rows ? (double)a.t_rows[r] : a.t;
+  const double mp = a.mp_rows ? (double)a.mp_rows[r] : a.mp;
+  Setting s;
+  s.p = a.p_rows ? (double)a.p_rows[r] : a.p;
+  s.k = a.k_rows ? a.k_rows[r] : a.k;
+  if (!(t > 0.0)) { t = 1.0; s.k = 1; }  // no temperature: the first of the largest
+  if (s.p <= 0.0) { s.p = 1.0; s.k = 1; }
+  s.sc = fmin(1.4426950408889634074 / t, 1e300);
+  s.least = mp > 0.0 ? fmin(mp, 1.0) * UNIT : 0.0;
+  s.u = a.u[r];
+  return s;
+}
+// the integer that the kept mass has to reach: mass > u * total
+__device__ __forceinline__ u64 draw_at(float uf, u64 total) {
+  const double u = uf > 0.0f ? fmin((double)uf, 1.0 - 1.0 / 9007199254740992.0) : 0.0;  // (NaN: 0)
+  const u64 d = (u64)(u * (double)total);
+  return d < total ? d + 1 : total;
+}
+// ceil(share of total): a member is kept whose mass before it is < share * total, so the prefix is the shortest whose mass reaches this
+__device__ __forceinline__ u64 share_of(double share, u64 total) {
+  const u64 need = (u64)ceil(share * (double)total);
+  return need > total ? total : need < 1 ? 1 : need;
+}
+__device__ __forceinline__ float logp_of(uint32_t key, double m, double sc, bool inf_row, u64 total) {
+  return (float)((inf_row ? 0.0 : ((double)score_of(key) - m) * (sc * 0.693147180559945309417)) - log((double)total / UNIT));
+}
 
-template <class T> struct Row {
+// ---------------------------------------------------------------------------------------------------- rows of up to 64 E scores
+// A lane holds E neighbours, so lanes are in index order.
+template <class T, int E> __global__ __launch_bounds__(256) void k_sample_wave(Args a, int rows) {
+  const int lane = threadIdx.x & 63, n = a.n;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= rows) return;
+  const T *row = (const T *)a.scores + r * a.stride;
+  const uint8_t *legal = a.legal ? a.legal + r * a.legal_stride : nullptr;
+  const Setting st = setting_of(a, r);
+  const int i0 = lane * E;
+  uint32_t key[E], kmax = KEY_NONE, kmin = 0xFFFFFFFFu;
+#pragma unroll
+  for (int j = 0; j < E; ++j) key[j] = i0 + j < n ? key_of(to_f32(row[i0 + j])) : KEY_NONE;
+  if (legal) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (i0 + j < n && legal[i0 + j] == 0) key[j] = KEY_NONE;
+  }
+  int left = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const bool on = key[j] != KEY_NONE;
+    kmax = key[j] > kmax ? key[j] : kmax;
+    kmin = on && key[j] < kmin ? key[j] : kmin;
+    left += __popcll(__ballot(on));
+  }
+  if (left == 0) {
+    if (lane == 0) {
+      a.actions[r] = -1;
+      if (a.logp) a.logp[r] = -INFINITY;
+    }
+    return;
+  }
+  kmax = wave_max(kmax);
+  const bool inf_row = kmax == KEY_PINF;
+  const double m = inf_row ? 0.0 : (double)score_of(kmax);
+  // the first `take` (in index order) of the scores equal to `tie`, and what is above it, stay
+  auto keep = [&](uint32_t tie, int take) {
+    uint32_t eq = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) eq += key[j] == tie;
+    uint32_t before = wave_scan(eq) - eq;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const bool is = key[j] == tie;
+      if (key[j] < tie || (is && before >= (uint32_t)take)) key[j] = KEY_NONE;
+      before += is;
+    }
+  };
+  // halfway between two keys: by value for the first steps (scores spread evenly by value), then by bits, which ends for certain
+  auto middle = [](uint32_t lo, uint32_t hi, int step) {
+    if (step < 16) {
+      const uint32_t v = key_of(0.5f * score_of(lo) + 0.5f * score_of(hi - 1));
+      if (v > lo && v < hi) return v;
+    }
+    return lo + (hi - lo) / 2;
+  };
+  const bool cut_k = st.k > 0 && st.k < left, cut_p = st.p < 1.0;
+  if (cut_k || cut_p) kmin = ~wave_max(~kmin);
+  if (cut_k) {  // count(>= lo) > k > count(>= hi), or the exact count
+    uint32_t lo = kmin, hi = kmax + 1;
+    int above = 0;
+    bool exact = false;
+    for (int step = 0; hi - lo > 1; ++step) {
+      const uint32_t mid = middle(lo, hi, step);
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) c += __popcll(__ballot(key[j] >= mid));
+      if (c > st.k) lo = mid;
+      else { hi = mid; above = c; }
+      if (c == st.k) { exact = true; break; }
+    }
+    if (exact) keep(hi - 1, 0);
+    else keep(lo, st.k - above);
+    left = st.k;
+  }
+  u64 w[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) w[j] = weight(key[j], m, st.sc, inf_row);
+  if (cut_p) {  // mass(>= lo) reaches the share, mass(>= hi) does not
+    u64 s = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) s += w[j];
+    const u64 need = share_of(st.p, wave_sum(s));
+    uint32_t lo = kmin, hi = kmax + 1;
+    u64 above = 0;
+    int c_lo = left, c_hi = 0;
+    for (int step = 0; hi - lo > 1 && c_lo - c_hi > 1; ++step) {
+      const uint32_t mid = middle(lo, hi, step);
+      u64 s = 0;
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool in = key[j] >= mid;
+        s += in ? w[j] : 0;
+        c += __popcll(__ballot(in));
+      }
+      s = wave_sum(s);
+      if (s >= need) { lo = mid; c_lo = c; }
+      else { hi = mid; above = s; c_hi = c; }
+    }
+    if (hi - lo > 1) keep(lo, 0x7FFFFFFF);  // one score in between: the last member
+    else {
+      const u64 each = weight(lo, m, st.sc, inf_row), take = (need - above + each - 1) / each;
+      keep(lo, take < 0x7FFFFFFF ? (int)take : 0x7FFFFFFF);
+    }
+  }
+  u64 mine = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if (key[j] == KEY_NONE || (double)w[j] < st.least) w[j] = 0;
+    mine += w[j];
+  }
+  const u64 incl = wave_scan(mine), total = lane_of(incl, 63), need = draw_at(st.u, total);
+  if (incl >= need && incl - mine < need) {
+    u64 run = incl - mine;
+    int at = 0;
+    uint32_t at_key = key[0];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if (run < need && run + w[j] >= need) { at = j; at_key = key[j]; }
+      run += w[j];
+    }
+    a.actions[r] = i0 + at;
+    if (a.logp) a.logp[r] = logp_of(at_key, m, st.sc, inf_row, total);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- longer rows
+// The row as the workgroup sees it: vectors of 16 bytes, vector v of thread t holds the scores from (v * NT + t) * V on; a walk reads
+// one vector ahead.  (Held in registers instead, every walk unrolls over all vectors: 20,000 instructions, and 1,024 threads spill.)
+// Masked scores and those behind the row's end are NaN.
+template <class T, int NT> struct Row {
+  static constexpr int V = 16 / sizeof(T), N = Word<T>::N;
   const T *s;
   const uint8_t *legal;
-  __device__ __forceinline__ uint32_t key(int i) const { return legal != nullptr && legal[i] == 0 ? KEY_NONE : key_of(to_f32(s[i])); }
+  int n, tid, walks;
+
+  __device__ __forceinline__ u32x4 read(int v) const {
+    const int i = (v * NT + tid) * V;
+    u32x4 w;
+    if (i + V <= n) __builtin_memcpy(&w, s + i, 16);
+    else {
+      T e[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        from_f32(NAN, e[j]);
+        if (i + j < n) e[j] = s[i + j];
+      }
+      __builtin_memcpy(&w, e, 16);
+    }
+    if (legal) {
+      uint8_t on[V];
+      if (i + V <= n) __builtin_memcpy(on, legal + i, V);
+      else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) on[j] = i + j < n ? legal[i + j] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j / N] |= on[j] ? 0u : N == 1 ? 0xFFFFFFFFu : 0xFFFFu << (16 * (j % N));  // (all ones: a NaN of any type)
+    }
+    return w;
+  }
+  // f(key, index) for every score of this thread, g(v) after every vector
+  template <class F, class G> __device__ __forceinline__ void walk(F f, G g) const {
+    u32x4 next = read(0);
+    for (int v = 0; v < walks; ++v) {
+      const u32x4 w = next;
+      if (v + 1 < walks) next = read(v + 1);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f(key_of(Word<T>::get(w[j / N], j % N)), (v * NT + tid) * V + j);
+      g(v);
+    }
+  }
+  template <class F> __device__ __forceinline__ void walk(F f) const { walk(f, [](int) {}); }
+};
+
+template <int NT> struct Shared {
+  u64 hist[BINS];
+  u64 part[NT / 64];
+  uint32_t kmax[NT / 64], kmin[NT / 64];
+  u64 base, value;
+  u64 list_w[LIST];
+  uint32_t list_key[LIST];
+  int32_t list_idx[LIST], bin, count;
+  uint32_t end_key;
+  int32_t end_idx;
 };
 
 struct Limit {  // the last member of a prefix of the order
@@ -106,13 +334,13 @@ struct Limit {  // the last member of a prefix of the order
 
 // Where the running sum of hist (bins in order) first reaches `need`: sh.bin (BINS: nowhere), sh.base = the sum before that bin,
 // sh.value = the bin's own.
-__device__ void find_bin(Shared &sh, u64 need, int tid) {
+template <int NT> __device__ __forceinline__ void find_bin(Shared<NT> &sh, u64 need, int tid) {
   constexpr int PER = BINS / NT;
   u64 mine = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) mine += sh.hist[tid * PER + j];
   const int lane = tid & 63, wave = tid >> 6;
-  const u64 incl = wave_scan(mine, lane);
+  const u64 incl = wave_scan(mine);
   if (lane == 63) sh.part[wave] = incl;
   if (tid == 0) sh.bin = BINS;
   __syncthreads();
@@ -134,13 +362,12 @@ __device__ void find_bin(Shared &sh, u64 need, int tid) {
 }
 
 // The shortest prefix of `in` (itself a prefix of the order) whose count reaches `need`, or (MASS) whose mass reaches the share
-// `frac` of `in`'s mass.  A prefix of the order keeps a member whose mass before it is < P: as masses are integers, that is the
-// shortest prefix whose mass is >= ceil(P).  First a histogram linear in the score (spreads the atomics), then histograms over the keys of the bin found,
-// 11 bits at a time, until a bin is one key; its equal scores are cut by index.
-template <class T, bool MASS>
-__device__ Limit cut(const Row<T> &row, int n, Shared &sh, Limit in, uint32_t kmax, uint32_t kmin, double m, double sc, bool inf_row,
-                     u64 need, double frac, int tid) {
-  const int lane = tid & 63, wave = tid >> 6;
+// `frac` of `in`'s mass.  A histogram linear in the score, then the scores of the bin found: as a list where they fit, each of which
+// sums what lies before it; else (thousands of nearly equal scores) histograms over their keys, 11 bits at a time, until a bin is one
+// key, whose equal scores are cut by index.
+template <bool MASS, int NT, class H>
+__device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uint32_t kmax, uint32_t kmin, double m, double sc, bool inf_row, u64 need, double frac) {
+  const int tid = row.tid, lane = tid & 63, wave = tid >> 6;
   const float top = score_of(kmax);
   float span = top - score_of(kmin);
   if (MASS) span = fminf(span, (float)(45.0 / sc));  // below 2^-45 of the largest there is no mass
@@ -149,17 +376,17 @@ __device__ Limit cut(const Row<T> &row, int n, Shared &sh, Limit in, uint32_t km
   u64 base = 0;
   bool linear = span > 0.0f && span < INFINITY && scale < INFINITY && kmax - kmin >= (uint32_t)BINS;
   if (!linear) klo = kmin;
+  auto bin_of = [&](uint32_t k) { return (int)fminf((top - score_of(k)) * scale, (float)(BINS - 1)); };
   for (;;) {
     for (int i = tid; i < BINS; i += NT) sh.hist[i] = 0;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
     const int bits = 32 - __clz((int)(khi - klo) | 1), shift = bits > 11 ? bits - 11 : 0;
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t k = row.key(i);
-      if (k == KEY_NONE || k > khi || k < klo || !in.has(k, i)) continue;
-      const int b = linear ? (int)fminf((top - score_of(k)) * scale, (float)(BINS - 1)) : (int)((khi - k) >> shift);
+    row.walk([&](uint32_t k, int i) {
+      if (k == KEY_NONE || k > khi || k < klo || !in.has(k, i)) return;
       const u64 v = MASS ? weight(k, m, sc, inf_row) : 1;
-      if (v) atomicAdd(&sh.hist[b], v);
-    }
+      if (v) atomicAdd(&sh.hist[linear ? bin_of(k) : (int)((khi - k) >> shift)], v);
+    });
     __syncthreads();
     if (MASS && frac > 0.0) {  // the first histogram holds the whole mass of `in`: the target is a share of it
       u64 s = 0;
@@ -168,34 +395,49 @@ __device__ Limit cut(const Row<T> &row, int n, Shared &sh, Limit in, uint32_t km
       if (lane == 0) sh.part[wave] = s;
       __syncthreads();
       s = 0;
-      for (int w = 0; w < WAVES; ++w) s += sh.part[w];
+      for (int w = 0; w < NT / 64; ++w) s += sh.part[w];
       __syncthreads();
-      need = (u64)ceil(frac * (double)s);  // frac < 1: at most the mass itself, but for the rounding
-      need = need > s ? s : need < 1 ? 1 : need;
+      need = share_of(frac, s);
       frac = 0.0;
     }
-    find_bin(sh, need - base, tid);
+    find_bin<NT>(sh, need - base, tid);
     if (sh.bin >= BINS) return in;  // never reached: nothing is cut
     const int b = sh.bin;
-    const u64 before = base + sh.base, value = sh.value;
+    const u64 value = sh.value;
+    base += sh.base;
     __syncthreads();
-    base = before;
-    if (linear) {  // the keys of that bin
+    if (linear) {
+      // the scores of that bin: their list, their number and the range of their keys
       uint32_t hi = KEY_NONE, lo = 0xFFFFFFFFu;
-      for (int i = tid; i < n; i += NT) {
-        const uint32_t k = row.key(i);
-        if (k == KEY_NONE || k > khi || !in.has(k, i)) continue;
-        if ((int)fminf((top - score_of(k)) * scale, (float)(BINS - 1)) != b) continue;
+      row.walk([&](uint32_t k, int i) {
+        if (k == KEY_NONE || !in.has(k, i) || bin_of(k) != b) return;
         hi = k > hi ? k : hi;
         lo = k < lo ? k : lo;
-      }
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < LIST) { sh.list_key[at] = k; sh.list_idx[at] = i; }
+      });
       hi = wave_max(hi);
       lo = ~wave_max(~lo);
       if (lane == 0) { sh.kmax[wave] = hi; sh.kmin[wave] = lo; }
       __syncthreads();
+      const int c = sh.count;
+      if (c <= LIST) {
+        for (int e = tid; e < c; e += NT) sh.list_w[e] = MASS ? weight(sh.list_key[e], m, sc, inf_row) : 1;
+        __syncthreads();
+        for (int e = tid; e < c; e += NT) {
+          const uint32_t k = sh.list_key[e];
+          const int i = sh.list_idx[e];
+          u64 before = base;
+          for (int x = 0; x < c; ++x)
+            if (sh.list_key[x] > k || (sh.list_key[x] == k && sh.list_idx[x] < i)) before += sh.list_w[x];
+          if (before < need && before + sh.list_w[e] >= need) { sh.end_key = k; sh.end_idx = i; }  // (one member)
+        }
+        __syncthreads();
+        return Limit{sh.end_key, sh.end_idx};
+      }
       khi = KEY_NONE;
       klo = 0xFFFFFFFFu;
-      for (int w = 0; w < WAVES; ++w) { khi = sh.kmax[w] > khi ? sh.kmax[w] : khi; klo = sh.kmin[w] < klo ? sh.kmin[w] : klo; }
+      for (int w = 0; w < NT / 64; ++w) { khi = sh.kmax[w] > khi ? sh.kmax[w] : khi; klo = sh.kmin[w] < klo ? sh.kmin[w] : klo; }
       __syncthreads();
       linear = false;
       continue;
@@ -211,44 +453,43 @@ __device__ Limit cut(const Row<T> &row, int n, Shared &sh, Limit in, uint32_t km
     const u64 each = MASS ? weight(tk, m, sc, inf_row) : 1, ties = value / each;  // (a bin that is reached holds mass)
     const u64 take = (need - base + each - 1) / each;
     if (take >= ties) return Limit{tk, tk == in.key ? in.idx : 0x7FFFFFFF};
-    // the index of the take-th equal score: counted in index order
-    if (tid == 0) sh.tie = -1;
-    __syncthreads();
+    // the index of the take-th equal score: counted in index order, a vector of every thread at a time
     u64 seen = 0;
-    for (int i0 = 0; i0 < n; i0 += NT) {
-      const int i = i0 + tid;
-      const bool eq = i < n && row.key(i) == tk;
-      const u64 mask = __ballot(eq);
-      if (lane == 0) sh.part[wave] = (u64)__popcll(mask);
-      __syncthreads();
-      u64 mine = seen, all = 0;
-      for (int w = 0; w < WAVES; ++w) { mine += w < wave ? sh.part[w] : 0; all += sh.part[w]; }
-      mine += (u64)__popcll(mask & ((2ull << lane) - 1));
-      if (eq && mine == take) sh.tie = i;
-      seen += all;
-      __syncthreads();
-      if (seen >= take) break;
-    }
-    return Limit{tk, sh.tie};
+    uint32_t mine = 0, mask = 0;
+    row.walk([&](uint32_t k, int i) { mine += k == tk; mask = (mask << 1) | (k == tk); },
+             [&](int v) {
+               if (seen < take) {  // (uniform)
+                 const uint32_t incl = wave_scan(mine);
+                 if (lane == 63) sh.part[wave] = incl;
+                 __syncthreads();
+                 u64 before = seen + incl - mine, all = 0;
+                 for (int w = 0; w < NT / 64; ++w) { before += w < wave ? sh.part[w] : 0; all += sh.part[w]; }
+                 if (before < take && before + mine >= take) {
+                   int left = (int)(take - before);
+                   for (int j = H::V - 1; j >= 0; --j)
+                     if (((mask >> j) & 1) && --left == 0) sh.end_idx = (v * NT + tid) * H::V + H::V - 1 - j;
+                 }
+                 seen += all;
+                 __syncthreads();
+               }
+               mine = mask = 0;
+             });
+    return Limit{tk, sh.end_idx};
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(NT) void k_sample_block(Args a) {
-  __shared__ Shared sh;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
-  const Row<T> row{(const T *)a.scores + (int64_t)r * a.stride, a.legal ? a.legal + (int64_t)r * a.legal_stride : nullptr};
-  double t = a.t_rows ? (double)a.t_rows[r] : a.t, p = a.p_rows ? (double)a.p_rows[r] : a.p, mp = a.mp_rows ? (double)a.mp_rows[r] : a.mp;
-  int k = a.k_rows ? a.k_rows[r] : a.k;
-  if (!(t > 0.0)) { t = 1.0; k = 1; }  // no temperature: the first of the largest
-  const double sc = fmin(1.4426950408889634074 / t, 1e300);
+template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(Args a) {
+  __shared__ Shared<NT> sh;
+  constexpr int WAVES = NT / 64, V = 16 / sizeof(T);
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, walks = (n + NT * V - 1) / (NT * V);
+  const Row<T, NT> row{(const T *)a.scores + r * a.stride, a.legal ? a.legal + r * a.legal_stride : nullptr, n, tid, walks};
+  const Setting st = setting_of(a, r);
   uint32_t kmax = KEY_NONE, kmin = 0xFFFFFFFFu;
-  for (int i = tid; i < n; i += NT) {
-    const uint32_t key = row.key(i);
-    if (key == KEY_NONE) continue;
-    kmax = key > kmax ? key : kmax;
-    kmin = key < kmin ? key : kmin;
-  }
+  row.walk([&](uint32_t k, int) {
+    kmax = k > kmax ? k : kmax;
+    kmin = k != KEY_NONE && k < kmin ? k : kmin;
+  });
   kmax = wave_max(kmax);
   kmin = ~wave_max(~kmin);
   if (lane == 0) { sh.kmax[wave] = kmax; sh.kmin[wave] = kmin; }
@@ -265,52 +506,68 @@ __global__ __launch_bounds__(NT) void k_sample_block(Args a) {
   const bool inf_row = kmax == KEY_PINF;
   const double m = inf_row ? 0.0 : (double)score_of(kmax);
   Limit lim{KEY_NONE, -1};
-  if (k > 0 && k < n) lim = cut<T, false>(row, n, sh, lim, kmax, kmin, m, sc, inf_row, (u64)k, 0.0, tid);
-  __syncthreads();
-  if (p < 1.0) {
-    if (p <= 0.0) lim = cut<T, false>(row, n, sh, lim, kmax, kmin, m, sc, inf_row, 1, 0.0, tid);
-    else lim = cut<T, true>(row, n, sh, lim, kmax, kmin, m, sc, inf_row, 0, p, tid);
+  if (st.k > 0 && st.k < n) {
+    lim = cut<false, NT>(row, sh, lim, kmax, kmin, m, st.sc, inf_row, (u64)st.k, 0.0);
     __syncthreads();
   }
-  const double least = mp > 0.0 ? fmin(mp, 1.0) * UNIT : 0.0;
-  // kept mass of every tile of NT indices, in index order
-  const int tiles = (n + NT - 1) / NT;
-  auto kept = [&](int i) -> u64 {
-    if (i >= n) return 0;
-    const uint32_t key = row.key(i);
-    if (key == KEY_NONE || !lim.has(key, i)) return 0;
-    const u64 w = weight(key, m, sc, inf_row);
-    return (double)w >= least ? w : 0;
-  };
-  for (int i = tid; i < BINS; i += NT) sh.hist[i] = 0;
-  __syncthreads();
-  for (int tile = 0; tile < tiles; ++tile) {
-    const u64 s = wave_sum(kept(tile * NT + tid));
-    if (lane == 0 && s) atomicAdd(&sh.hist[tile], s);
+  if (st.p < 1.0) {
+    lim = cut<true, NT>(row, sh, lim, kmax, kmin, m, st.sc, inf_row, 0, st.p);
+    __syncthreads();
   }
+  auto kept = [&](uint32_t k, int i) -> u64 {
+    if (k == KEY_NONE || !lim.has(k, i)) return 0;
+    const u64 w = weight(k, m, st.sc, inf_row);
+    return (double)w >= st.least ? w : 0;
+  };
+  // kept mass of every wave's share of every vector, in index order: walks * WAVES sums, at most 2^19 / (64 V) = 2,048
+  u64 mine = 0;
+  row.walk([&](uint32_t k, int i) { mine += kept(k, i); },
+           [&](int v) {
+             const u64 s = wave_sum(mine);
+             if (lane == 0) sh.hist[v * WAVES + wave] = s;
+             mine = 0;
+           });
+  const int sums = walks * WAVES;
+  for (int i = sums + tid; i < BINS; i += NT) sh.hist[i] = 0;
   __syncthreads();
   u64 total = 0;
-  for (int i = 0; i < tiles; i += 64) total += wave_sum(i + lane < tiles ? sh.hist[i + lane] : 0);
-  const float uf = a.u[r];
-  const double u = uf > 0.0f ? fmin((double)uf, 1.0 - 1.0 / 9007199254740992.0) : 0.0;  // (NaN: 0)
-  const u64 drawn = (u64)(u * (double)total), need = drawn < total ? drawn + 1 : total;  // mass > u * total, in integers
-  int tile = 0;
-  u64 before = 0;
-  while (before + sh.hist[tile] < need) before += sh.hist[tile++];  // (uniform; ends: need <= total)
-  const int i = tile * NT + tid;
-  const u64 w = kept(i);
-  u64 incl = wave_scan(w, lane);
-  if (lane == 63) sh.part[wave] = incl;
-  __syncthreads();
-  incl += before;
-  for (int x = 0; x < wave; ++x) incl += sh.part[x];
-  if (incl >= need && incl - w < need) sh.tie = i;
-  __syncthreads();
-  if (tid == 0) {
-    const int at = sh.tie;
-    a.actions[r] = at;
-    if (a.logp) a.logp[r] = (float)((inf_row ? 0.0 : ((double)score_of(row.key(at)) - m) * (sc * 0.693147180559945309417)) - log((double)total / UNIT));
+  for (int i = lane; i < sums; i += 64) total += sh.hist[i];
+  total = wave_sum(total);
+  const u64 need = draw_at(st.u, total);
+  find_bin<NT>(sh, need, tid);  // (a bin is found: need <= total)
+  if (sh.bin % WAVES != wave) return;
+  const int v = sh.bin / WAVES;
+  const u32x4 words = row.read(v);
+  u64 w[V];
+  mine = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = kept(key_of(Word<T>::get(words[j / Word<T>::N], j % Word<T>::N)), (v * NT + tid) * V + j);
+    mine += w[j];
   }
+  u64 run = sh.base + wave_scan(mine) - mine;
+  if (run < need && run + mine >= need) {
+    for (int j = 0; j < V; ++j) {
+      if (run < need && run + w[j] >= need) {
+        const int at = (v * NT + tid) * V + j;
+        a.actions[r] = at;
+        if (a.logp) a.logp[r] = logp_of(key_of(to_f32(row.s[at])), m, st.sc, inf_row, total);
+      }
+      run += w[j];
+    }
+  }
+}
+
+// the kernel that holds a row of n scores
+template <class T> static void launch(const Args &a, int rows, hipStream_t s) {
+  const dim3 four((rows + 3) / 4), one(rows);
+  if (a.n <= 64) hipLaunchKernelGGL((k_sample_wave<T, 1>), four, dim3(256), 0, s, a, rows);
+  else if (a.n <= 128) hipLaunchKernelGGL((k_sample_wave<T, 2>), four, dim3(256), 0, s, a, rows);
+  else if (a.n <= 256) hipLaunchKernelGGL((k_sample_wave<T, 4>), four, dim3(256), 0, s, a, rows);
+  else if (a.n <= 512) hipLaunchKernelGGL((k_sample_wave<T, 8>), four, dim3(256), 0, s, a, rows);
+  else if (a.n <= 1024) hipLaunchKernelGGL((k_sample_wave<T, 16>), four, dim3(256), 0, s, a, rows);
+  else if (a.n <= 8192) hipLaunchKernelGGL((k_sample_block<T, 256>), one, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_sample_block<T, 1024>), one, dim3(1024), 0, s, a);
 }
 
 }  // namespace azsample
@@ -336,8 +593,8 @@ extern "C" int az_sample_actions(int32_t dtype, int32_t rows, int32_t n, const v
   if (!guard.ok) return fail(AZ_EHIP, "sample: cannot select the stream's device");
   Args a{scores_dev, legal_dev, uniforms_dev, temperature_dev, top_p_dev, min_p_dev, top_k_dev, actions_dev, logprobs_dev,
          row_stride, legal_stride, temperature, top_p, min_p, top_k, n};
-  if (dtype == AZ_NN_F32) hipLaunchKernelGGL(k_sample_block<float>, dim3(rows), dim3(NT), 0, s, a);
-  else if (dtype == AZ_NN_BF16) hipLaunchKernelGGL(k_sample_block<bf16_t>, dim3(rows), dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL(k_sample_block<f16_t>, dim3(rows), dim3(NT), 0, s, a);
+  if (dtype == AZ_NN_F32) launch<float>(a, rows, s);
+  else if (dtype == AZ_NN_BF16) launch<bf16_t>(a, rows, s);
+  else launch<f16_t>(a, rows, s);
   return launched("k_sample");
 }
