@@ -13,10 +13,12 @@
 // The kept set is a prefix of the order, so it is described by its last member (key, index), and no row is ever sorted.
 //
 //   n <= 1,024: a row is one wave's, in registers; the prefix's end is bisected over the score, counting with ballots
-//   longer:     a row is one workgroup's, which walks it a few times (after the first time it comes from the caches); the prefix's
-//               end comes from a histogram linear in the score and a list of the scores in the bin it falls into
+//   longer:     a row is one workgroup's, which walks it twice where it can (the second time it comes from the caches): the first
+//               walk leaves every thread's largest score; what nine sixteenths of these reach (or k of them, for the top k), some 0.8 scores
+//               a thread do where large scores lie anywhere; the second walk lists those in LDS and bounds the mass in f32.  If the prefix ends within the list, the list is sorted and the rest is done on
+//               it.  A longer prefix is found from a histogram linear in the score and a list of the bin it ends in.
 //
-// Bound by the exponentials: about 25 f64 operations each, at most two per score (the mass of the whole row, the kept mass).
+// Bound by instructions: about ten a score and walk, and 25 f64 operations an exponential where the kept scores are many.
 #include "az_ops.hip.h"
 
 namespace azsample {
@@ -48,29 +50,41 @@ __device__ __forceinline__ uint32_t key_of(float s) {
 }
 __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key); }
 
-// 2^44 exp((s - m) / T) rounded to an integer; sc = log2(e) / T.  2^f on [-1/2, 1/2] by its Taylor polynomial of degree 12
-// (remainder below 2^-51); scores of +inf share the whole mass.
-__device__ __forceinline__ u64 weight(uint32_t key, double m, double sc, bool inf_row) {
-  if (key == KEY_NONE) return 0;
-  if (inf_row) return key == KEY_PINF ? (u64)UNIT : 0;
-  double y = ((double)score_of(key) - m) * sc;
-  y = y < -100.0 ? -100.0 : y;
-  const double kf = rint(y), f = (y - kf) * 0.693147180559945309417;
-  double r = 1.0 / 479001600.0;
-  r = fma(r, f, 1.0 / 39916800.0);
-  r = fma(r, f, 1.0 / 3628800.0);
-  r = fma(r, f, 1.0 / 362880.0);
-  r = fma(r, f, 1.0 / 40320.0);
-  r = fma(r, f, 1.0 / 5040.0);
-  r = fma(r, f, 1.0 / 720.0);
-  r = fma(r, f, 1.0 / 120.0);
-  r = fma(r, f, 1.0 / 24.0);
-  r = fma(r, f, 1.0 / 6.0);
-  r = fma(r, f, 0.5);
-  r = fma(r, f, 1.0);
-  r = fma(r, f, 1.0);
+// 2^44 exp((s - m) / T) rounded to an integer, of N scores side by side (they share the constants and fill each other's latencies);
+// sc = log2(e) / T.  2^f on [-1/2, 1/2] by its Taylor polynomial of degree 12 (remainder below 2^-51); scores of +inf share the whole
+// mass.
+template <int N> __device__ __forceinline__ void weights(const uint32_t *key, double m, double sc, bool inf_row, u64 *w) {
+  if (inf_row) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = key[j] == KEY_PINF ? (u64)UNIT : 0;
+    return;
+  }
+  double f[N], r[N];
+  int e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const double y = __builtin_fmax(((double)score_of(key[j]) - m) * sc, -100.0), k = rint(y);
+    f[j] = (y - k) * 0.693147180559945309417;
+    e[j] = (int)k + 44;
+    r[j] = 1.0 / 479001600.0;
+  }
+  constexpr double C[12] = {1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+  for (int d = 0; d < 12; ++d) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r[j] = fma(r[j], f[j], C[d]);
+  }
   // 2^52 + w: the integer stands in the low mantissa bits, rounded to nearest even (w <= 2^44)
-  return (u64)__double_as_longlong(ldexp(r, (int)kf + 44) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const u64 v = (u64)__double_as_longlong(ldexp(r[j], e[j]) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    w[j] = key[j] == KEY_NONE ? 0 : v;
+  }
+}
+__device__ __forceinline__ u64 weight(uint32_t key, double m, double sc, bool inf_row) {
+  u64 w;
+  weights<1>(&key, m, sc, inf_row, &w);
+  return w;
 }
 
 // Wave reductions by data-parallel moves (rows of 16 lanes, then across rows): no LDS round trips.  The result is in lane 63 of a scan.
@@ -137,6 +151,15 @@ __device__ __forceinline__ float logp_of(uint32_t key, double m, double sc, bool
   return (float)((inf_row ? 0.0 : ((double)score_of(key) - m) * (sc * 0.693147180559945309417)) - log((double)total / UNIT));
 }
 
+// halfway between two keys: by value for the first steps (scores spread evenly by value), then by bits, which ends for certain
+__device__ __forceinline__ uint32_t middle(uint32_t lo, uint32_t hi, int step) {
+  if (step < 16) {
+    const uint32_t v = key_of(0.5f * score_of(lo) + 0.5f * score_of(hi - 1));
+    if (v > lo && v < hi) return v;
+  }
+  return lo + (hi - lo) / 2;
+}
+
 // ---------------------------------------------------------------------------------------------------- rows of up to 64 E scores
 // A lane holds E neighbours, so lanes are in index order.
 template <class T, int E> __global__ __launch_bounds__(256) void k_sample_wave(Args a, int rows) {
@@ -186,14 +209,6 @@ template <class T, int E> __global__ __launch_bounds__(256) void k_sample_wave(A
       before += is;
     }
   };
-  // halfway between two keys: by value for the first steps (scores spread evenly by value), then by bits, which ends for certain
-  auto middle = [](uint32_t lo, uint32_t hi, int step) {
-    if (step < 16) {
-      const uint32_t v = key_of(0.5f * score_of(lo) + 0.5f * score_of(hi - 1));
-      if (v > lo && v < hi) return v;
-    }
-    return lo + (hi - lo) / 2;
-  };
   const bool cut_k = st.k > 0 && st.k < left, cut_p = st.p < 1.0;
   if (cut_k || cut_p) kmin = ~wave_max(~kmin);
   if (cut_k) {  // count(>= lo) > k > count(>= hi), or the exact count
@@ -214,8 +229,9 @@ template <class T, int E> __global__ __launch_bounds__(256) void k_sample_wave(A
     left = st.k;
   }
   u64 w[E];
+  constexpr int SIDE = E < 4 ? E : 4;
 #pragma unroll
-  for (int j = 0; j < E; ++j) w[j] = weight(key[j], m, st.sc, inf_row);
+  for (int j = 0; j < E; j += SIDE) weights<SIDE>(key + j, m, st.sc, inf_row, w + j);
   if (cut_p) {  // mass(>= lo) reaches the share, mass(>= hi) does not
     u64 s = 0;
 #pragma unroll
@@ -279,13 +295,13 @@ template <class T, int NT> struct Row {
     const int i = (v * NT + tid) * V;
     u32x4 w;
     if (i + V <= n) __builtin_memcpy(&w, s + i, 16);
-    else {
+    else {  // the row's last vector, and those behind it: every load at once, from inside the row
       T e[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        from_f32(NAN, e[j]);
-        if (i + j < n) e[j] = s[i + j];
-      }
+      for (int j = 0; j < V; ++j) e[j] = s[min(i + j, n - 1)];
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i + j >= n) from_f32(NAN, e[j]);
       __builtin_memcpy(&w, e, 16);
     }
     if (legal) {
@@ -293,25 +309,33 @@ template <class T, int NT> struct Row {
       if (i + V <= n) __builtin_memcpy(on, legal + i, V);
       else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) on[j] = i + j < n ? legal[i + j] : 0;
+        for (int j = 0; j < V; ++j) on[j] = legal[min(i + j, n - 1)];
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) w[j / N] |= on[j] ? 0u : N == 1 ? 0xFFFFFFFFu : 0xFFFFu << (16 * (j % N));  // (all ones: a NaN of any type)
     }
     return w;
   }
-  // f(key, index) for every score of this thread, g(v) after every vector
-  template <class F, class G> __device__ __forceinline__ void walk(F f, G g) const {
+  // f(keys of a vector, index of its first score, vector), all lanes together.  (Four vectors ahead instead of one gains nothing: a walk
+  // is bound by its instructions.)
+  template <class F> __device__ __forceinline__ void walk(F f) const {
     u32x4 next = read(0);
     for (int v = 0; v < walks; ++v) {
       const u32x4 w = next;
       if (v + 1 < walks) next = read(v + 1);
+      uint32_t k[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) f(key_of(Word<T>::get(w[j / N], j % N)), (v * NT + tid) * V + j);
-      g(v);
+      for (int j = 0; j < V; ++j) k[j] = key_of(Word<T>::get(w[j / N], j % N));
+      f(k, (v * NT + tid) * V, v);
     }
   }
-  template <class F> __device__ __forceinline__ void walk(F f) const { walk(f, [](int) {}); }
+};
+
+// a listed score: its place in the order as one number (key, then the lower index first), and its mass
+struct alignas(16) Member {
+  u64 rank, w;
+  __device__ __forceinline__ uint32_t key() const { return (uint32_t)(rank >> 32); }
+  __device__ __forceinline__ int idx() const { return (int)~(uint32_t)rank; }
 };
 
 template <int NT> struct Shared {
@@ -319,11 +343,11 @@ template <int NT> struct Shared {
   u64 part[NT / 64];
   uint32_t kmax[NT / 64], kmin[NT / 64];
   u64 base, value;
-  u64 list_w[LIST];
-  uint32_t list_key[LIST];
-  int32_t list_idx[LIST], bin, count;
-  uint32_t end_key;
-  int32_t end_idx;
+  Member list[LIST];
+  Member end;
+  u64 end_upto;
+  int32_t bin, count, end_idx;
+  uint32_t reached;
 };
 
 struct Limit {  // the last member of a prefix of the order
@@ -361,12 +385,74 @@ template <int NT> __device__ __forceinline__ void find_bin(Shared<NT> &sh, u64 n
   __syncthreads();
 }
 
+// Appends the keys of a vector that bits of `on` name: one addition to the count a wave.  Called by all lanes; beyond LIST the count goes
+// on and nothing is stored.
+template <int V, int NT> __device__ __forceinline__ void append(Shared<NT> &sh, uint32_t on, const uint32_t *key, int idx) {
+  if (__ballot(on != 0) == 0) return;
+  const uint32_t mine = __popc(on), incl = wave_scan(mine);
+  int at = 0;
+  if ((threadIdx.x & 63) == 63) at = atomicAdd(&sh.count, (int)incl);
+  at = __builtin_amdgcn_readlane(at, 63) + (int)(incl - mine);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if ((on >> j) & 1) {
+      if (at < LIST) sh.list[at].rank = ((u64)key[j] << 32) | (uint32_t)~(idx + j);
+      ++at;
+    }
+}
+
+template <int NT> __device__ __forceinline__ u64 block_sum(Shared<NT> &sh, u64 v, int tid) {
+  v = wave_sum(v);
+  if ((tid & 63) == 0) sh.part[tid >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < NT / 64; ++w) v += sh.part[w];
+  __syncthreads();
+  return v;
+}
+
+// Where the running sum of the list's masses, in the order that `ahead` tells and `bin_of` follows, first reaches need (at most their
+// sum): sh.end, and the sum up to and with it in sh.end_upto.  A histogram, then the members of one bin, each of which sums what of
+// them lies ahead of it.
+template <int NT, class B, class A> __device__ __forceinline__ void list_find(Shared<NT> &sh, int c, u64 need, int tid, B bin_of, A ahead) {
+  for (int i = tid; i < BINS; i += NT) sh.hist[i] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  for (int e = tid; e < c; e += NT) {
+    const Member m = sh.list[e];
+    if (m.w) atomicAdd(&sh.hist[bin_of(m)], m.w);
+  }
+  __syncthreads();
+  find_bin<NT>(sh, need, tid);
+  const int b = sh.bin;
+  const u64 base = sh.base;
+  Member *own = (Member *)sh.hist;  // (the sums have been read)
+  static_assert(sizeof(Member) * LIST <= sizeof(sh.hist), "a bin's members fit the histogram's memory");
+  for (int e = tid; e < c; e += NT) {
+    const Member m = sh.list[e];
+    if (m.w && bin_of(m) == b) own[atomicAdd(&sh.count, 1)] = m;
+  }
+  __syncthreads();
+  const int n = sh.count;
+  for (int e = tid; e < n; e += NT) {
+    const Member me = own[e];
+    u64 upto = base + me.w;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const Member o = own[x];
+      upto += ahead(o, me) ? o.w : 0;
+    }
+    if (upto >= need && upto - me.w < need) { sh.end = me; sh.end_upto = upto; }  // (one member)
+  }
+  __syncthreads();
+}
+
 // The shortest prefix of `in` (itself a prefix of the order) whose count reaches `need`, or (MASS) whose mass reaches the share
-// `frac` of `in`'s mass.  A histogram linear in the score, then the scores of the bin found: as a list where they fit, each of which
-// sums what lies before it; else (thousands of nearly equal scores) histograms over their keys, 11 bits at a time, until a bin is one
-// key, whose equal scores are cut by index.
+// `frac` of `in`'s mass.  A histogram linear in the score, then a list of the bin found; where that does not fit (thousands of nearly
+// equal scores), histograms over their keys, 11 bits at a time, until a bin is one key, whose equal scores are cut by index.
 template <bool MASS, int NT, class H>
 __device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uint32_t kmax, uint32_t kmin, double m, double sc, bool inf_row, u64 need, double frac) {
+  constexpr int V = H::V;
   const int tid = row.tid, lane = tid & 63, wave = tid >> 6;
   const float top = score_of(kmax);
   float span = top - score_of(kmin);
@@ -382,21 +468,21 @@ __device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uin
     if (tid == 0) sh.count = 0;
     __syncthreads();
     const int bits = 32 - __clz((int)(khi - klo) | 1), shift = bits > 11 ? bits - 11 : 0;
-    row.walk([&](uint32_t k, int i) {
-      if (k == KEY_NONE || k > khi || k < klo || !in.has(k, i)) return;
-      const u64 v = MASS ? weight(k, m, sc, inf_row) : 1;
-      if (v) atomicAdd(&sh.hist[linear ? bin_of(k) : (int)((khi - k) >> shift)], v);
+    row.walk([&](const uint32_t *k, int i, int) {
+      bool on[V];
+      u64 w[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) on[j] = k[j] != KEY_NONE && k[j] <= khi && k[j] >= klo && in.has(k[j], i + j);
+      if (MASS) weights<V>(k, m, sc, inf_row, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (on[j] && (!MASS || w[j])) atomicAdd(&sh.hist[linear ? bin_of(k[j]) : (int)((khi - k[j]) >> shift)], MASS ? w[j] : 1);
     });
     __syncthreads();
     if (MASS && frac > 0.0) {  // the first histogram holds the whole mass of `in`: the target is a share of it
       u64 s = 0;
       for (int i = tid; i < BINS; i += NT) s += sh.hist[i];
-      s = wave_sum(s);
-      if (lane == 0) sh.part[wave] = s;
-      __syncthreads();
-      s = 0;
-      for (int w = 0; w < NT / 64; ++w) s += sh.part[w];
-      __syncthreads();
+      s = block_sum<NT>(sh, s, tid);
       need = share_of(frac, s);
       frac = 0.0;
     }
@@ -407,14 +493,18 @@ __device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uin
     base += sh.base;
     __syncthreads();
     if (linear) {
-      // the scores of that bin: their list, their number and the range of their keys
+      // the scores of that bin: their list, and the range of their keys
       uint32_t hi = KEY_NONE, lo = 0xFFFFFFFFu;
-      row.walk([&](uint32_t k, int i) {
-        if (k == KEY_NONE || !in.has(k, i) || bin_of(k) != b) return;
-        hi = k > hi ? k : hi;
-        lo = k < lo ? k : lo;
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < LIST) { sh.list_key[at] = k; sh.list_idx[at] = i; }
+      row.walk([&](const uint32_t *k, int i, int) {
+        uint32_t on = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (k[j] != KEY_NONE && in.has(k[j], i + j) && bin_of(k[j]) == b) {
+            hi = k[j] > hi ? k[j] : hi;
+            lo = k[j] < lo ? k[j] : lo;
+            on |= 1u << j;
+          }
+        append<V, NT>(sh, on, k, i);
       });
       hi = wave_max(hi);
       lo = ~wave_max(~lo);
@@ -422,18 +512,14 @@ __device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uin
       __syncthreads();
       const int c = sh.count;
       if (c <= LIST) {
-        for (int e = tid; e < c; e += NT) sh.list_w[e] = MASS ? weight(sh.list_key[e], m, sc, inf_row) : 1;
+        for (int e = tid; e < c; e += NT) sh.list[e].w = MASS ? weight(sh.list[e].key(), m, sc, inf_row) : 1;
         __syncthreads();
-        for (int e = tid; e < c; e += NT) {
-          const uint32_t k = sh.list_key[e];
-          const int i = sh.list_idx[e];
-          u64 before = base;
-          for (int x = 0; x < c; ++x)
-            if (sh.list_key[x] > k || (sh.list_key[x] == k && sh.list_idx[x] < i)) before += sh.list_w[x];
-          if (before < need && before + sh.list_w[e] >= need) { sh.end_key = k; sh.end_idx = i; }  // (one member)
-        }
-        __syncthreads();
-        return Limit{sh.end_key, sh.end_idx};
+        uint32_t first_key = KEY_NONE;
+        for (int w = 0; w < NT / 64; ++w) first_key = max(first_key, sh.kmax[w]);
+        const float first = score_of(first_key), fine = fminf((float)BINS * scale, 3e38f);
+        list_find<NT>(sh, c, need - base, tid, [&](const Member &x) { return (int)fminf((first - score_of(x.key())) * fine, (float)(BINS - 1)); },
+                      [](const Member &x, const Member &me) { return x.rank > me.rank; });
+        return Limit{sh.end.key(), sh.end.idx()};
       }
       khi = KEY_NONE;
       klo = 0xFFFFFFFFu;
@@ -455,25 +541,22 @@ __device__ __forceinline__ Limit cut(const H &row, Shared<NT> &sh, Limit in, uin
     if (take >= ties) return Limit{tk, tk == in.key ? in.idx : 0x7FFFFFFF};
     // the index of the take-th equal score: counted in index order, a vector of every thread at a time
     u64 seen = 0;
-    uint32_t mine = 0, mask = 0;
-    row.walk([&](uint32_t k, int i) { mine += k == tk; mask = (mask << 1) | (k == tk); },
-             [&](int v) {
-               if (seen < take) {  // (uniform)
-                 const uint32_t incl = wave_scan(mine);
-                 if (lane == 63) sh.part[wave] = incl;
-                 __syncthreads();
-                 u64 before = seen + incl - mine, all = 0;
-                 for (int w = 0; w < NT / 64; ++w) { before += w < wave ? sh.part[w] : 0; all += sh.part[w]; }
-                 if (before < take && before + mine >= take) {
-                   int left = (int)(take - before);
-                   for (int j = H::V - 1; j >= 0; --j)
-                     if (((mask >> j) & 1) && --left == 0) sh.end_idx = (v * NT + tid) * H::V + H::V - 1 - j;
-                 }
-                 seen += all;
-                 __syncthreads();
-               }
-               mine = mask = 0;
-             });
+    row.walk([&](const uint32_t *k, int i, int) {
+      if (seen >= take) return;  // (uniform)
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) mine += k[j] == tk;
+      const uint32_t incl = wave_scan(mine);
+      if (lane == 63) sh.part[wave] = incl;
+      __syncthreads();
+      u64 before = seen + incl - mine, all = 0;
+      for (int w = 0; w < NT / 64; ++w) { before += w < wave ? sh.part[w] : 0; all += sh.part[w]; }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (k[j] == tk && ++before == take) sh.end_idx = i + j;
+      seen += all;
+      __syncthreads();
+    });
     return Limit{tk, sh.end_idx};
   }
 }
@@ -485,16 +568,16 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, walks = (n + NT * V - 1) / (NT * V);
   const Row<T, NT> row{(const T *)a.scores + r * a.stride, a.legal ? a.legal + r * a.legal_stride : nullptr, n, tid, walks};
   const Setting st = setting_of(a, r);
-  uint32_t kmax = KEY_NONE, kmin = 0xFFFFFFFFu;
-  row.walk([&](uint32_t k, int) {
-    kmax = k > kmax ? k : kmax;
-    kmin = k != KEY_NONE && k < kmin ? k : kmin;
+  uint32_t kmax = KEY_NONE;
+  row.walk([&](const uint32_t *k, int, int) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) kmax = k[j] > kmax ? k[j] : kmax;
   });
+  const uint32_t own_max = kmax;
   kmax = wave_max(kmax);
-  kmin = ~wave_max(~kmin);
-  if (lane == 0) { sh.kmax[wave] = kmax; sh.kmin[wave] = kmin; }
+  if (lane == 0) sh.kmax[wave] = kmax;
   __syncthreads();
-  for (int w = 0; w < WAVES; ++w) { kmax = sh.kmax[w] > kmax ? sh.kmax[w] : kmax; kmin = sh.kmin[w] < kmin ? sh.kmin[w] : kmin; }
+  for (int w = 0; w < WAVES; ++w) kmax = sh.kmax[w] > kmax ? sh.kmax[w] : kmax;
   __syncthreads();
   if (kmax == KEY_NONE) {  // nothing legal
     if (tid == 0) {
@@ -505,28 +588,157 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   }
   const bool inf_row = kmax == KEY_PINF;
   const double m = inf_row ? 0.0 : (double)score_of(kmax);
+  const bool cut_k = st.k > 0 && st.k < n, cut_p = st.p < 1.0;
+  if ((cut_k || cut_p) && !(cut_k && st.k > LIST)) {
+    // the largest key that nine sixteenths of the threads' largest reach, or, for the top k, that k of them do (all legal scores, if too few hold any)
+    uint32_t *tops = (uint32_t *)sh.hist;
+    tops[tid] = own_max;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t top[NT / 64], lo = 0xFFFFFFFFu, hi = kmax + 1;
+      const int want = cut_k && st.k < NT * 9 / 16 ? st.k : NT * 9 / 16;
+#pragma unroll
+      for (int j = 0; j < NT / 64; ++j) {
+        top[j] = tops[j * 64 + lane];
+        lo = min(lo, top[j]);
+      }
+      lo = ~wave_max(~lo);
+      for (int step = 0; hi - lo > 1; ++step) {
+        const uint32_t mid = lo == KEY_NONE ? lo + (hi - lo) / 2 : middle(lo, hi, step);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < NT / 64; ++j) c += __popcll(__ballot(top[j] >= mid));
+        if (c >= want) lo = mid;
+        else hi = mid;
+        if (c == want) break;
+      }
+      if (lane == 0) sh.reached = lo == KEY_NONE ? KEY_NONE + 1 : lo;
+    }
+    __syncthreads();
+    const uint32_t reached = sh.reached;
+    // The mass of the row to within a share OFF, from f32 exponentials: (s - m) sc carries three roundings of 2^-24 of itself, at most 40
+    // before a weight is below 2^-40 (and all such together below 2^-21), the exponential 2^-22.  Where that does not settle where the
+    // prefix ends (a few rows in a hundred), the mass is summed exactly.
+    constexpr double OFF = 0x1p-17;
+    const float mf = score_of(kmax), scf = (float)st.sc;
+    const bool rough = !cut_k && !inf_row && scf < 1e30f;
+    double part = 0.0;
+    row.walk([&](const uint32_t *k, int i, int) {
+      uint32_t on = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) on |= k[j] >= reached ? 1u << j : 0;
+      append<V, NT>(sh, on, k, i);
+      if (rough) {
+        float w = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) w += __builtin_amdgcn_exp2f((score_of(k[j]) - mf) * scf);
+        part += (double)w;
+      }
+    });
+    u64 mass = block_sum<NT>(sh, (u64)(part * UNIT), tid);
+    int c = sh.count;
+    __syncthreads();
+    bool ends = c <= LIST && (!cut_k || c >= st.k || reached == KEY_NONE + 1);  // the prefix ends within the list
+    if (ends) {
+      const float top = score_of(kmax), scale = fminf((float)BINS / (top - score_of(reached)), 3e38f);  // (NaN and infinity: the first or the last bin)
+      auto in_order = [](const Member &x, const Member &me) { return x.rank > me.rank; };
+      auto by_score = [&](const Member &x) { return (int)fminf((top - score_of(x.key())) * scale, (float)(BINS - 1)); };
+      u64 last = 0;  // the place of the prefix's last member
+      if (cut_k && c > st.k) {
+        for (int e = tid; e < c; e += NT) sh.list[e].w = 1;
+        __syncthreads();
+        list_find<NT>(sh, c, (u64)st.k, tid, by_score, in_order);
+        last = sh.end.rank;
+      }
+      u64 sum = 0;
+      for (int e = tid; e < c; e += NT) sum += sh.list[e].w = sh.list[e].rank >= last ? weight(sh.list[e].key(), m, st.sc, inf_row) : 0;
+      sum = block_sum<NT>(sh, sum, tid);
+      if (cut_p) {
+        u64 need = share_of(st.p, sum);
+        bool found = false;
+        if (!cut_k && rough) {
+          need = share_of(st.p, (u64)((double)mass * (1.0 - OFF)));
+          ends = sum >= need;
+          if (ends) {
+            list_find<NT>(sh, c, need, tid, by_score, in_order);
+            found = share_of(st.p, (u64)((double)mass * (1.0 + OFF))) <= sh.end_upto;
+          }
+        }
+        if (ends && !found) {
+          if (!cut_k) {
+            mass = 0;
+            row.walk([&](const uint32_t *k, int, int) {
+              u64 w[V];
+              weights<V>(k, m, st.sc, inf_row, w);
+#pragma unroll
+              for (int j = 0; j < V; ++j) mass += w[j];
+            });
+            need = share_of(st.p, block_sum<NT>(sh, mass, tid));
+            ends = sum >= need;
+          }
+          if (ends) list_find<NT>(sh, c, need, tid, by_score, in_order);
+        }
+        last = sh.end.rank;
+      }
+      if (ends) {
+        sum = 0;
+        for (int e = tid; e < c; e += NT) {
+          Member &x = sh.list[e];
+          if (x.rank < last || (double)x.w < st.least) x.w = 0;
+          sum += x.w;
+        }
+        const u64 total = block_sum<NT>(sh, sum, tid);
+        const int shift = 32 - __clz((n - 1) | 1) > 11 ? 32 - __clz((n - 1) | 1) - 11 : 0;
+        list_find<NT>(sh, c, draw_at(st.u, total), tid, [&](const Member &x) { return x.idx() >> shift; },
+                      [](const Member &x, const Member &me) { return x.idx() < me.idx(); });
+        if (tid == 0) {
+          a.actions[r] = sh.end.idx();
+          if (a.logp) a.logp[r] = logp_of(sh.end.key(), m, st.sc, inf_row, total);
+        }
+        return;
+      }
+    }
+    __syncthreads();
+  }
   Limit lim{KEY_NONE, -1};
-  if (st.k > 0 && st.k < n) {
+  uint32_t kmin = 0xFFFFFFFFu;
+  if (cut_k || cut_p) {
+    row.walk([&](const uint32_t *k, int, int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) kmin = min(kmin, k[j] - (KEY_NONE + 1));  // (KEY_NONE wraps to the top)
+    });
+    kmin = ~wave_max(~kmin);
+    if (lane == 0) sh.kmin[wave] = kmin;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) kmin = min(kmin, sh.kmin[w]);
+    kmin += KEY_NONE + 1;
+    __syncthreads();
+  }
+  if (cut_k) {
     lim = cut<false, NT>(row, sh, lim, kmax, kmin, m, st.sc, inf_row, (u64)st.k, 0.0);
     __syncthreads();
   }
-  if (st.p < 1.0) {
+  if (cut_p) {
     lim = cut<true, NT>(row, sh, lim, kmax, kmin, m, st.sc, inf_row, 0, st.p);
     __syncthreads();
   }
-  auto kept = [&](uint32_t k, int i) -> u64 {
-    if (k == KEY_NONE || !lim.has(k, i)) return 0;
-    const u64 w = weight(k, m, st.sc, inf_row);
-    return (double)w >= st.least ? w : 0;
-  };
   // kept mass of every wave's share of every vector, in index order: walks * WAVES sums, at most 2^19 / (64 V) = 2,048
-  u64 mine = 0;
-  row.walk([&](uint32_t k, int i) { mine += kept(k, i); },
-           [&](int v) {
-             const u64 s = wave_sum(mine);
-             if (lane == 0) sh.hist[v * WAVES + wave] = s;
-             mine = 0;
-           });
+  auto kept_of = [&](const uint32_t *k, int i, u64 *w) {  // -> their sum
+    weights<V>(k, m, st.sc, inf_row, w);
+    u64 s = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!lim.has(k[j], i + j) || (double)w[j] < st.least) w[j] = 0;
+      s += w[j];
+    }
+    return s;
+  };
+  row.walk([&](const uint32_t *k, int i, int v) {
+    u64 w[V];
+    const u64 s = wave_sum(kept_of(k, i, w));
+    if (lane == 0) sh.hist[v * WAVES + wave] = s;
+  });
   const int sums = walks * WAVES;
   for (int i = sums + tid; i < BINS; i += NT) sh.hist[i] = 0;
   __syncthreads();
@@ -538,20 +750,18 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   if (sh.bin % WAVES != wave) return;
   const int v = sh.bin / WAVES;
   const u32x4 words = row.read(v);
+  uint32_t keys[V];
   u64 w[V];
-  mine = 0;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = kept(key_of(Word<T>::get(words[j / Word<T>::N], j % Word<T>::N)), (v * NT + tid) * V + j);
-    mine += w[j];
-  }
+  for (int j = 0; j < V; ++j) keys[j] = key_of(Word<T>::get(words[j / Word<T>::N], j % Word<T>::N));
+  const u64 mine = kept_of(keys, (v * NT + tid) * V, w);
   u64 run = sh.base + wave_scan(mine) - mine;
   if (run < need && run + mine >= need) {
+#pragma unroll
     for (int j = 0; j < V; ++j) {
       if (run < need && run + w[j] >= need) {
-        const int at = (v * NT + tid) * V + j;
-        a.actions[r] = at;
-        if (a.logp) a.logp[r] = logp_of(key_of(to_f32(row.s[at])), m, st.sc, inf_row, total);
+        a.actions[r] = (v * NT + tid) * V + j;
+        if (a.logp) a.logp[r] = logp_of(keys[j], m, st.sc, inf_row, total);
       }
       run += w[j];
     }
