@@ -53,15 +53,18 @@ template <class T> __device__ __forceinline__ void put_param(void *p, int f32, i
   else from_f32((float)v, ((T *)p)[i]);
 }
 
-struct Stat {  // of one group, as the elementwise part uses it
-  float mh, ml, rs;
+// of one group, as the elementwise part uses it: xhat = (x - mean) rstd with the mean as a pair of f32, (x - mh) rs + off
+struct Stat {
+  float mh, off, rs;
+  __device__ __forceinline__ float xhat(float x) const { return fmaf(x - mh, rs, off); }
 };
 __device__ __forceinline__ Stat stat_of(double mean, double rstd) {
   const float mh = (float)mean;
-  return Stat{mh, (float)(mean - (double)mh), (float)rstd};
+  return Stat{mh, (float)(((double)mh - mean) * rstd), (float)rstd};
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + expf(-z)); }
+// 1 / (1 + 2^(-z log2 e)): off by |z| 2^-23 of itself at most where it is small, which z sigmoid(z) and the gradient share
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
 
 // the activation of V values; `act` is uniform, so this is one branch for all of them
 template <int V> __device__ __forceinline__ void act_fwd(float *z, int act) {
@@ -79,7 +82,7 @@ template <int V> __device__ __forceinline__ void act_fwd(float *z, int act) {
 template <int V, bool RES> __device__ __forceinline__ void grad(const float *x, const float *r, const float *w, const float *b, const Stat &st,
                                                                 const double *sd, int act, float *d, float *xh) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) xh[j] = ((x[j] - st.mh) - st.ml) * st.rs;
+  for (int j = 0; j < V; ++j) xh[j] = st.xhat(x[j]);
   if (act == AZ_ACT_RELU) {
     float z[V];
     bool unsure = false;
@@ -135,6 +138,7 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_stats(Args 
     const int col = c0 + k.tx;
     double s = 0.0, q = 0.0;
     if (col < k.cv && k.ty < k.ty_n)
+#pragma unroll 4
       for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
         float v[V];
         load<T, V>(v, x + (int64_t)p * a.c + col * V);
@@ -190,13 +194,14 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_apply(Args 
     float w[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+#pragma unroll 2
     for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
       const int64_t at = base + (int64_t)p * a.c + col * V;
       float v[V], r[V] = {};
       load<T, V>(v, (const T *)a.x + at);
       if (a.r) load<T, V>(r, (const T *)a.r + at);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = fmaf(((v[j] - s.mh) - s.ml) * s.rs, w[j], b[j]) + r[j];
+      for (int j = 0; j < V; ++j) v[j] = fmaf(s.xhat(v[j]), w[j], b[j]) + r[j];
       act_fwd<V>(v, a.act);
       store<T, V>((T *)a.y + at, v);
     }
@@ -219,6 +224,7 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_sums(Ar
       float w[V], b[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+#pragma unroll 2
       for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
         const int64_t at = base + (int64_t)p * a.c + col * V;
         float x[V], r[V] = {}, d[V];
@@ -300,6 +306,7 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args
     float w[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+#pragma unroll 2
     for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
       const int64_t at = base + (int64_t)p * a.c + col * V;
       float x[V], r[V] = {}, d[V];
@@ -384,7 +391,7 @@ template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_
     if (RES) unpack<T>(rv[i], rf);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      f[j] = fmaf(((f[j] - st.mh) - st.ml) * st.rs, w[j], b[j]);
+      f[j] = fmaf(st.xhat(f[j]), w[j], b[j]);
       if (RES) f[j] += rf[j];
     }
     act_fwd<V>(f, a.act);
@@ -471,7 +478,7 @@ template <class T, int NV, bool RES, int ACT> __global__ __launch_bounds__(NT) v
       dv[i] = pack<T>(d);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) xh[j] = ((xf[j] - st.mh) - st.ml) * st.rs;
+      for (int j = 0; j < V; ++j) xh[j] = st.xhat(xf[j]);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) xf[j] = st.rs * (fmaf(d[j], w[j], -m1) - xh[j] * m2);
@@ -481,24 +488,29 @@ template <class T, int NV, bool RES, int ACT> __global__ __launch_bounds__(NT) v
   }
 }
 
-// the samples' channel sums -> dweight, dbias: 16 channels x 16 samples a workgroup.  Beyond 4,096 samples in `splits` shares (LAST
-// false: into wpart), joined by a second pass.
-template <class T, bool LAST> __global__ __launch_bounds__(NT) void k_gn_wb(Args a) {
-  __shared__ double s_[NT], q_[NT];
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+// the samples' channel sums -> dweight, dbias: 4 channels (32 bytes of a row) x 256 rows at a time a workgroup.  Beyond 4,096 samples in
+// `splits` shares (LAST false: into wpart), joined by a second pass.
+constexpr int WB_C = 4, WB_NT = 1024;
+template <class T, bool LAST> __global__ __launch_bounds__(WB_NT) void k_gn_wb(Args a) {
+  __shared__ double s_[WB_NT / 64][WB_C], q_[WB_NT / 64][WB_C];
+  const int tid = threadIdx.x, c = blockIdx.x * WB_C + tid % WB_C, lane = tid / WB_C;
   const bool joined = LAST && a.splits > 1;
   const int64_t rows = joined ? a.splits : a.n, per = LAST ? rows : (rows + a.splits - 1) / a.splits;
   const int64_t r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
   double s = 0.0, q = 0.0;
   if (c < a.c) {
-    if (joined) for (int64_t r = r0 + lane; r < r1; r += 16) { const double *p = a.wpart + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
-    else for (int64_t r = r0 + lane; r < r1; r += 16) { const float *p = a.csum + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
+    if (joined) for (int64_t r = r0 + lane; r < r1; r += WB_NT / WB_C) { const double *p = a.wpart + (r * a.c + c) * 2; s += p[0]; q += p[1]; }
+    else {
+#pragma unroll 4
+      for (int64_t r = r0 + lane; r < r1; r += WB_NT / WB_C) { const float2 p = *(const float2 *)(a.csum + (r * a.c + c) * 2); s += p.x; q += p.y; }
+    }
   }
-  s_[threadIdx.x] = s;
-  q_[threadIdx.x] = q;
+  for (int o = WB_C; o < 64; o <<= 1) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
+  if ((tid & 63) < WB_C) { s_[tid >> 6][tid % WB_C] = s; q_[tid >> 6][tid % WB_C] = q; }
   __syncthreads();
-  if (lane != 0 || c >= a.c) return;
-  for (int l = 1; l < 16; ++l) { s += s_[l * 16 + threadIdx.x]; q += q_[l * 16 + threadIdx.x]; }
+  if (tid >= WB_C || c >= a.c) return;
+  s = q = 0.0;
+  for (int w = 0; w < WB_NT / 64; ++w) { s += s_[w][tid]; q += q_[w][tid]; }
   if (LAST) {
     put_param<T>(a.db, a.param_f32, c, s);
     put_param<T>(a.dw, a.param_f32, c, q);
@@ -509,9 +521,10 @@ template <class T, bool LAST> __global__ __launch_bounds__(NT) void k_gn_wb(Args
   }
 }
 
-// pixels of a sample are shared out so that there are workgroups enough, but never fewer than 32 pixels to one
+// pixels of a sample are shared out so that there are workgroups enough (four a CU; eight are no faster and leave twice the partial sums
+// to join), but never fewer than 32 pixels to one
 static int chunks_of(int64_t n, int hw) {
-  int64_t want = (2048 + n - 1) / n, most = (hw + 31) / 32;
+  int64_t want = (1024 + n - 1) / n, most = (hw + 31) / 32;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 static int splits_of(int64_t n) { return n <= 4096 ? 1 : n < 65536 ? (int)(n / 1024) : 64; }
@@ -680,7 +693,7 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
     a.n = 0;
     a.splits = 1;
     return by_dtype(dtype, [&](auto t) {
-      hipLaunchKernelGGL((k_gn_wb<decltype(t), true>), dim3((c + 15) / 16), dim3(NT), 0, s, a);
+      hipLaunchKernelGGL((k_gn_wb<decltype(t), true>), dim3((c + WB_C - 1) / WB_C), dim3(WB_NT), 0, s, a);
       return launched("k_gn_wb");
     });
   }
@@ -727,8 +740,8 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
   if (rc != AZ_OK || !params) return rc;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.splits > 1) hipLaunchKernelGGL((k_gn_wb<T, false>), dim3((c + 15) / 16, a.splits), dim3(NT), 0, s, a);
-    hipLaunchKernelGGL((k_gn_wb<T, true>), dim3((c + 15) / 16), dim3(NT), 0, s, a);
+    if (a.splits > 1) hipLaunchKernelGGL((k_gn_wb<T, false>), dim3((c + WB_C - 1) / WB_C, a.splits), dim3(WB_NT), 0, s, a);
+    hipLaunchKernelGGL((k_gn_wb<T, true>), dim3((c + WB_C - 1) / WB_C), dim3(WB_NT), 0, s, a);
     return launched("k_gn_wb");
   });
 }

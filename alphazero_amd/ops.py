@@ -22,6 +22,21 @@ def _stream(device: torch.device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _on:
+    """the device current for the allocations inside, without a switch where it is current already"""
+
+    def __init__(self, device: torch.device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def _on_gpu(t: torch.Tensor, name: str, dtypes=None, device=None) -> None:
     if not isinstance(t, torch.Tensor):
         raise EngineError(f"{name}: expected a tensor, got {type(t).__name__}")
@@ -77,7 +92,7 @@ def sample_actions(scores: torch.Tensor, uniforms: torch.Tensor, *, temperature=
     m_t, m_v = _per_row(min_p, "min_p", rows, torch.float32, dev)
     if not (t_v >= 0 and k_v >= 0 and p_v >= 0 and 0 <= m_v <= 1) or k_v != int(k_v):
         raise EngineError("temperature >= 0, top_k >= 0 (a whole number), top_p >= 0 and 0 <= min_p <= 1")
-    with torch.cuda.device(dev):
+    with _on(dev):
         actions = torch.empty(rows, dtype=torch.int32, device=dev)
         logp = torch.empty(rows, dtype=torch.float32, device=dev) if return_logprobs else None
         _check(load_library().az_sample_actions(
@@ -116,7 +131,7 @@ class _GroupNormAct(torch.autograd.Function):
         weight = weight.contiguous() if weight is not None else None
         bias = bias.contiguous() if bias is not None else None
         pd = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             y = _empty_like(x)
             stats = torch.empty((n, groups, 2), dtype=torch.float64, device=x.device)
             ws = _workspace(0, n, h * w, c, groups, x.device)
@@ -134,7 +149,7 @@ class _GroupNormAct(torch.autograd.Function):
         n, c, h, w = x.shape
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dy = _dense(dy)
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             dx = _empty_like(x) if need_x else None
             dw = torch.empty(c, dtype=ctx.pd, device=x.device) if need_w else None
             db = torch.empty(c, dtype=ctx.pd, device=x.device) if need_b else None
@@ -211,7 +226,7 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.
     if not ms:
         return torch.empty_like(matrices) if single else []
     lib, dev, n = load_library(), ms[0].device, len(ms)
-    with torch.cuda.device(dev):
+    with _on(dev):
         src = [m.contiguous() for m in ms]
         out = torch.empty(matrices.shape, dtype=matrices.dtype, device=dev) if single else [torch.empty(m.shape, dtype=m.dtype, device=dev) for m in ms]
         dst = out if not single else [out] if matrices.dim() == 2 else list(out.unbind(0))
