@@ -381,6 +381,248 @@ template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds
   }
 }
 
+// ---------------------------------------------------------------------------------------------------- one workgroup a matrix
+// A short side of at most 64 and a long one of at most 768: X stays in registers for all steps (f32, 32 x 32 blocks as the matrix
+// instructions leave them: a lane holds a column's rows in groups of four), eight waves own every eighth column block.  Nothing but A
+// and B passes through LDS, and one launch replaces 17: those matrices' steps are bound by launches and latencies.
+//   B X: the block's own rows are the second factor as they lie; the first (rows of B) is read in the same order of k.
+//   X X^T needs X with a lane holding a row: the block times the identity, which moves every f16 half unchanged.
+// Partial sums of A go through LDS (four waves' at a time, always added in one order), waves 0 .. 2 take a tile of A and B each.
+constexpr int SMALL_S = 64, SMALL_L = 768, SMALL_NT = 512, SMALL_NB = 3;
+
+struct SmallTable {
+  Mat m[MAX_M];
+};
+
+// piece q (four halves) of row r of a 64 x 64 f16 plane; the pieces of 16 rows fall on different banks
+__device__ __forceinline__ int piece(int r, int q) { return r * 64 + ((q ^ (r & 15)) << 2); }
+
+template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_os_small(SmallTable t, float ca, float cb, float cc, double eps, float sx, float sa, float sb, int steps) {
+  constexpr int TILES = RB == 1 ? 1 : 3;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILES * 16 * 64 * 4 + 64 * 64 * 2 * P];
+  float *part = (float *)lds;                                         // [slot 4][tile][element 16][lane]
+  _Float16 *am = (_Float16 *)(lds + 4 * TILES * 16 * 64 * 4);         // A: planes of 64 x 64
+  _Float16 *bm = (_Float16 *)lds;                                     // B: over the partial sums, which have been read by then
+  static_assert(64 * 64 * 2 * P <= 4 * TILES * 16 * 64 * 4, "B fits the partial sums' memory");
+  const Mat m = t.m[blockIdx.x];
+  const bool tall = m.rows > m.cols;
+  const int S = tall ? m.cols : m.rows, L = tall ? m.rows : m.cols;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, l32 = lane & 31;
+  const int blocks = (L + 31) / 32, nb = wave < blocks ? (blocks - wave + 7) / 8 : 0;
+  f32x16 x[SMALL_NB][RB];
+  double sum = 0.0;
+#pragma unroll
+  for (int b = 0; b < SMALL_NB; ++b)
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = (wave + 8 * b) * 32 + l32, i = r * 32 + (e >> 2) * 8 + hf * 4 + (e & 3);
+        float v = 0.0f;
+        if (b < nb && j < L && i < S) v = to_f32(((const E *)m.in)[(uint32_t)(tall ? j * S + i : i * L + j)]);
+        x[b][r][e] = v;
+        sum = fma((double)v, (double)v, sum);
+      }
+  {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    double *s_ = (double *)lds;
+    if (lane == 0) s_[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < 8; ++w) sum += s_[w];
+    __syncthreads();
+  }
+  const double norm = sqrt(sum) + eps;
+  const double scale = norm < 1e300 ? (norm > 0.0 ? (double)sx / norm : 0.0) : NAN;  // (no finite norm: no result)
+#pragma unroll
+  for (int b = 0; b < SMALL_NB; ++b)
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = (wave + 8 * b) * 32 + l32, i = r * 32 + (e >> 2) * 8 + hf * 4 + (e & 3);
+        x[b][r][e] = b < nb && j < L && i < S ? (float)((double)x[b][r][e] * scale) : 0.0f;
+      }
+  int row4 = hf * 4, col = l32;
+  asm volatile("" : "+v"(row4), "+v"(col));  // (the stores compute their addresses again instead of keeping the loads')
+  // the identity in the order of k that a block's rows have: place (hf, j) of chunk c is row 16 c + (j / 4) * 8 + hf * 4 + j % 4
+  half8 one[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) one[c][j] = (_Float16)(16 * c + (j >> 2) * 8 + hf * 4 + (j & 3) == l32 ? 1.0f : 0.0f);
+  // plane h of 16 rows (chunk c) of a block
+  auto half_of = [&](const f32x16 &v, int c, int h) {
+    half8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const _Float16 hi = (_Float16)v[c * 8 + j];
+      o[j] = h == 0 ? hi : (_Float16)(v[c * 8 + j] - (float)hi);
+    }
+    return o;
+  };
+  // rows r * 32 .. of a symmetric 64 x 64 plane pair as the first factor, chunk c of its columns in that order of k
+  auto rows_of = [&](const _Float16 *p, int r, int c, int h) {
+    const _Float16 *q = p + h * 4096;
+    const half4 u = *(const half4 *)(q + piece(r * 32 + l32, c * 4 + hf)), v = *(const half4 *)(q + piece(r * 32 + l32, c * 4 + 2 + hf));
+    return half8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+  };
+  // a tile of a symmetric matrix into the planes: columns (four consecutive rows a lane), and off the diagonal its mirror image
+  auto put_tile = [&](_Float16 *p, const float *v, int ti, int tj) {
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      half4 hi, lo;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        hi[d] = (_Float16)v[e4 * 4 + d];
+        lo[d] = (_Float16)(v[e4 * 4 + d] - (float)hi[d]);
+      }
+      const int j = tj * 32 + l32, i = ti * 32 + e4 * 8 + hf * 4;
+      *(half4 *)(p + piece(j, i >> 2)) = hi;
+      if (P == 2) *(half4 *)(p + 4096 + piece(j, i >> 2)) = lo;
+      if (ti != tj) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          p[piece(i + d, j >> 2) + (j & 3)] = hi[d];
+          if (P == 2) p[4096 + piece(i + d, j >> 2) + (j & 3)] = lo[d];
+        }
+      }
+    }
+  };
+  for (int step = 0; step < steps; ++step) {
+    // A's share of this wave's columns
+    f32x16 acc[TILES] = {};
+#pragma unroll
+    for (int b = 0; b < SMALL_NB; ++b) {
+      if (b >= nb) continue;
+      half8 xt[RB][2][P];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int h = 0; h < P; ++h) {
+          f32x16 d = {};
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(x[b][r], 0, h), one[0], d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(x[b][r], 1, h), one[1], d, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xt[r][c][h][j] = (_Float16)d[c * 8 + j];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+      for (int q = 0; q < TILES; ++q) {
+        const int ti = q == 2 ? 1 : 0, tj = q == 0 ? 0 : 1;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (P == 2) {
+            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][P - 1], xt[RB == 1 ? 0 : tj][c][0], acc[q], 0, 0, 0);
+            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][0], xt[RB == 1 ? 0 : tj][c][P - 1], acc[q], 0, 0, 0);
+          }
+          acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][0], xt[RB == 1 ? 0 : tj][c][0], acc[q], 0, 0, 0);
+        }
+      }
+    }
+    __syncthreads();  // (B of the step before has been read)
+    auto slot = [&](int q, int e) { return part + (((wave & 3) * TILES + q) * 16 + e) * 64 + lane; };
+    if (wave >= 4) {
+#pragma unroll
+      for (int q = 0; q < TILES; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) *slot(q, e) = acc[q][e];
+    }
+    __syncthreads();
+    if (wave < 4) {
+#pragma unroll
+      for (int q = 0; q < TILES; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) *slot(q, e) += acc[q][e];
+    }
+    __syncthreads();
+    const int ti = wave == 2 ? 1 : 0, tj = wave == 0 || RB == 1 ? 0 : 1;  // waves 0 .. TILES - 1: their tile
+    float a[16];
+    if (wave < TILES) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float v = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) v += part[((s * TILES + wave) * 16 + e) * 64 + lane];
+        a[e] = v * (sa / (sx * sx));
+      }
+      put_tile(am, a, ti, tj);
+    }
+    __syncthreads();
+    if (wave < TILES) {
+      f32x16 d = {};
+#pragma unroll
+      for (int c = 0; c < 2 * RB; ++c) {
+        half8 p[P], q[P];
+#pragma unroll
+        for (int h = 0; h < P; ++h) { p[h] = rows_of(am, ti, c, h); q[h] = rows_of(am, tj, c, h); }
+        if (P == 2) {
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], q[0], d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], q[P - 1], d, 0, 0, 0);
+        }
+        d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], q[0], d, 0, 0, 0);
+      }
+      const float f = cc * (sb / (sa * sa)), g = cb * (sb / sa);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) a[e] = fmaf(f, d[e], g * a[e]);
+      put_tile(bm, a, ti, tj);
+    }
+    __syncthreads();
+    // X <- a X + B X
+    const float inv = 1.0f / sb;
+#pragma unroll
+    for (int b = 0; b < SMALL_NB; ++b)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) asm volatile("" : "+v"(x[b][r]));  // (or the halves made for A are all kept until here)
+#pragma unroll
+    for (int b = 0; b < SMALL_NB; ++b) {
+      if (b >= nb) continue;
+      half8 f[RB][2][P];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int h = 0; h < P; ++h) f[r][c][h] = half_of(x[b][r], c, h);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        f32x16 d = {};
+#pragma unroll
+        for (int c = 0; c < 2 * RB; ++c) {
+          half8 p[P];
+#pragma unroll
+          for (int h = 0; h < P; ++h) p[h] = rows_of(bm, r, c, h);
+          if (P == 2) {
+            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], f[c >> 1][c & 1][0], d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], f[c >> 1][c & 1][P - 1], d, 0, 0, 0);
+          }
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], f[c >> 1][c & 1][0], d, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[b][r][e] = fmaf(ca, x[b][r][e], d[e] * inv);
+      }
+    }
+  }
+  const float inv = 1.0f / sx;
+#pragma unroll
+  for (int b = 0; b < SMALL_NB; ++b)
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = (wave + 8 * b) * 32 + col, i = r * 32 + (e >> 2) * 8 + row4 + (e & 3);
+        if (b < nb && j < L && i < S) from_f32(x[b][r][e] * inv, ((E *)m.out)[(uint32_t)(tall ? j * S + i : i * L + j)]);
+      }
+}
+
+static bool is_small(int rows, int cols) {
+  const int s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+  return s <= SMALL_S && l <= SMALL_L;
+}
+
 static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }
 
 // tile side by the short side: measured on 1536 x 1536 / 2000 x 4096, 64 takes 0.47 / 1.54 ms in f32 and 0.25 / 0.76 ms in bf16, 128 takes
@@ -394,6 +636,14 @@ static int shares_of(const Lay &y, int tile) {
   if (tile != 64 || tiles > 96 || stages < 32) return 1;
   const int s = 512 / tiles < stages / 8 ? 512 / tiles : stages / 8;
   return s < 8 ? s : 8;
+}
+
+// One workgroup a matrix where every matrix of the call is small; beside larger ones they cost nothing in the others' launches, and a
+// launch of their own would (64 x 576 alone: 88 us in 17 launches, see above for one).
+static bool all_small(int count, const int32_t *rows, const int32_t *cols) {
+  for (int i = 0; i < count; ++i)
+    if (rows[i] > 0 && cols[i] > 0 && !is_small(rows[i], cols[i])) return false;
+  return true;
 }
 
 static int check(const char *&msg, int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols) {
@@ -473,6 +723,22 @@ template <class F> static int each_run(int planes, int count, const void *const 
   return AZ_OK;
 }
 
+template <class E, int P> static int run_small(const Args &a, int steps, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, hipStream_t s) {
+  for (int rb = 1; rb <= 2; ++rb) {
+    SmallTable t;
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+      const int side = rows[i] < cols[i] ? rows[i] : cols[i];
+      if (side > 0 && (side <= 32) == (rb == 1)) t.m[n++] = Mat{in[i], out[i], 0, rows[i], cols[i]};
+      if (n == 0 || (n < MAX_M && i < count - 1)) continue;
+      if (rb == 1) hipLaunchKernelGGL((k_os_small<E, P, 1>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
+      else hipLaunchKernelGGL((k_os_small<E, P, 2>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
+      n = 0;
+    }
+  }
+  return launched("k_os_small");
+}
+
 template <class E, int P, int T> static int run(const Run &r, Args a, int steps, hipStream_t s) {
   int64_t most = 0;
   for (int i = 0; i < r.t.count; ++i) {
@@ -513,6 +779,7 @@ int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *
   using namespace azortho;
   const char *msg = "";
   if (check(msg, dtype, count, rows, cols) != AZ_OK) { fail(AZ_EINVAL, msg); return -1; }
+  if (all_small(count, rows, cols)) return 0;
   uint64_t most = 0;  // (runs follow each other on the stream: they share the memory)
   each_run(dtype == AZ_NN_BF16 ? 1 : 2, count, nullptr, nullptr, rows, cols, [&](const Run &r) {
     most = r.bytes > most ? r.bytes : most;
@@ -539,13 +806,17 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
     if (!in[i] || !out[i] || misaligned(in[i], es) || misaligned(out[i], es)) return fail(AZ_EINVAL, "orthogonalize: null or misaligned matrix");
   }
   if (live == 0) return AZ_OK;
-  if (!workspace_dev || misaligned(workspace_dev, 256) || workspace_bytes < az_orthogonalize_workspace(dtype, count, rows, cols))
+  const bool small = all_small(count, rows, cols);
+  if (!small && (!workspace_dev || misaligned(workspace_dev, 256) || workspace_bytes < az_orthogonalize_workspace(dtype, count, rows, cols)))
     return fail(AZ_EINVAL, "orthogonalize: workspace below az_orthogonalize_workspace() or not aligned to 256 bytes");
   hipStream_t s = (hipStream_t)stream;
   DeviceGuard guard(s);
   if (!guard.ok) return fail(AZ_EHIP, "orthogonalize: cannot select the stream's device");
   g.ws = (char *)workspace_dev;
   g.a = (float)a; g.b = (float)b; g.c = (float)c; g.eps = eps;
+  if (small)
+    return dtype == AZ_NN_F32 ? run_small<float, 2>(g, steps, count, in, out, rows, cols, s) : dtype == AZ_NN_BF16 ? run_small<bf16_t, 1>(g, steps, count, in, out, rows, cols, s)
+                                                                                                                  : run_small<f16_t, 2>(g, steps, count, in, out, rows, cols, s);
   return each_run(planes, count, in, out, rows, cols, [&](const Run &r) {
     if (r.tile == 64) return dtype == AZ_NN_F32 ? run<float, 2, 64>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 64>(r, g, steps, s) : run<f16_t, 2, 64>(r, g, steps, s);
     return dtype == AZ_NN_F32 ? run<float, 2, 128>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 128>(r, g, steps, s) : run<f16_t, 2, 128>(r, g, steps, s);

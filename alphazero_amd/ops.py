@@ -203,7 +203,7 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.
 
     ``matrices``: a tensor (rows, cols), a batch (n, rows, cols), or a sequence of (rows, cols) tensors of any sizes, all f32, all
     bf16 or all f16, on one GPU -> new dense tensors of the same shapes and type (a sequence gives a list).  A whole network's
-    matrices in one call cost little more launches than one.  f32 and f16 results are accurate to f32 arithmetic, bf16 ones to
+    matrices in one call take no more launches than one.  f32 and f16 results are accurate to f32 arithmetic, bf16 ones to
     about their own rounding.  A matrix that holds an infinity or a NaN gives NaN.  Not differentiable."""
     single = isinstance(matrices, torch.Tensor)
     if single and matrices.dim() not in (2, 3):

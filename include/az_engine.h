@@ -491,7 +491,8 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
  * halves), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
  * under which a singular value in [0, 1] could grow beyond 7.5 are refused.
  * workspace_dev: az_orthogonalize_workspace() bytes (-1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
- * time need one each.  Matrices are independent: a matrix's result does not depend on the others in the call. */
+ * time need one each.  A matrix's result depends on the others in the call by its last bits at most: calls of matrices no larger than
+ * 64 x 768 alone take another kernel (and no workspace). */
 int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols);
 int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols,
                      int32_t steps, double a, double b, double c, double eps, void *workspace_dev, int64_t workspace_bytes, void *stream);

@@ -126,7 +126,7 @@ def test_norm_python_refusals_on_the_gpu():
 
 
 def _ortho(lib, **kw):
-    a = dict(dtype=0, count=1, ins=[512], outs=[512], rows=[4], cols=[5], steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, ws=512, size=1 << 24)
+    a = dict(dtype=0, count=1, ins=[512], outs=[512], rows=[100], cols=[200], steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, ws=512, size=1 << 24)
     a.update(kw)
     n = len(a["ins"])
     return lib.az_orthogonalize(a["dtype"], a["count"], (C.c_void_p * n)(*a["ins"]), (C.c_void_p * n)(*a["outs"]), (C.c_int32 * n)(*a["rows"]),
