@@ -382,8 +382,8 @@ template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds
 }
 
 // ---------------------------------------------------------------------------------------------------- one workgroup a matrix
-// A short side of at most 64 and a long one of at most 768: X stays in registers for all steps (f32, 32 x 32 blocks as the matrix
-// instructions leave them: a lane holds a column's rows in groups of four), eight waves own every eighth column block.  Nothing but A
+// A short side of at most 64 and a long one of at most 768: X stays in registers for all steps (its f16 halves, in 32 x 32 blocks as the
+// matrix instructions leave them: a lane holds a column's rows in groups of four), eight waves own every eighth column block.  Nothing but A
 // and B passes through LDS, and one launch replaces 17: those matrices' steps are bound by launches and latencies.
 //   B X: the block's own rows are the second factor as they lie; the first (rows of B) is read in the same order of k.
 //   X X^T needs X with a lane holding a row: the block times the identity, which moves every f16 half unchanged.
@@ -409,7 +409,8 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
   const int S = tall ? m.cols : m.rows, L = tall ? m.rows : m.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, l32 = lane & 31;
   const int blocks = (L + 31) / 32, nb = wave < blocks ? (blocks - wave + 7) / 8 : 0;
-  f32x16 x[SMALL_NB][RB];
+  u32x4 x[SMALL_NB][RB][2][P];  // [block][32 rows][chunk of 16 rows][hi, lo], two f16 a word
+  f32x16 raw[SMALL_NB][RB];
   double sum = 0.0;
 #pragma unroll
   for (int b = 0; b < SMALL_NB; ++b)
@@ -418,9 +419,9 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int j = (wave + 8 * b) * 32 + l32, i = r * 32 + (e >> 2) * 8 + hf * 4 + (e & 3);
-        float v = 0.0f;
-        if (b < nb && j < L && i < S) v = to_f32(((const E *)m.in)[(uint32_t)(tall ? j * S + i : i * L + j)]);
-        x[b][r][e] = v;
+        const int jc = min(j, L - 1), ic = min(i, S - 1);  // (every load at once, from inside the matrix)
+        const float in = to_f32(((const E *)m.in)[(uint32_t)(tall ? jc * S + ic : ic * L + jc)]), v = j < L && i < S ? in : 0.0f;
+        raw[b][r][e] = v;
         sum = fma((double)v, (double)v, sum);
       }
   {
@@ -435,33 +436,36 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
   }
   const double norm = sqrt(sum) + eps;
   const double scale = norm < 1e300 ? (norm > 0.0 ? (double)sx / norm : 0.0) : NAN;  // (no finite norm: no result)
+  typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
+  auto keep = [&](u32x4 (&o)[2][P], int e, float v0, float v1) {  // elements e and e + 1
+    const half2_ hi = {(_Float16)v0, (_Float16)v1};
+    o[e >> 3][0][(e & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
+    if (P == 2) o[e >> 3][P - 1][(e & 7) >> 1] = __builtin_bit_cast(uint32_t, half2_{(_Float16)(v0 - (float)hi[0]), (_Float16)(v1 - (float)hi[1])});
+  };
+  auto packed = [&](u32x4 (&o)[2][P]) {  // (whole words from here on, not an element a register)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int h = 0; h < P; ++h) asm volatile("" : "+v"(o[c][h]));
+  };
 #pragma unroll
   for (int b = 0; b < SMALL_NB; ++b)
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int r = 0; r < RB; ++r) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < 16; e += 2) {
         const int j = (wave + 8 * b) * 32 + l32, i = r * 32 + (e >> 2) * 8 + hf * 4 + (e & 3);
-        x[b][r][e] = b < nb && j < L && i < S ? (float)((double)x[b][r][e] * scale) : 0.0f;
+        const bool in = b < nb && j < L;
+        keep(x[b][r], e, in && i < S ? (float)((double)raw[b][r][e] * scale) : 0.0f, in && i + 1 < S ? (float)((double)raw[b][r][e + 1] * scale) : 0.0f);
       }
-  int row4 = hf * 4, col = l32;
-  asm volatile("" : "+v"(row4), "+v"(col));  // (the stores compute their addresses again instead of keeping the loads')
+      packed(x[b][r]);
+    }
   // the identity in the order of k that a block's rows have: place (hf, j) of chunk c is row 16 c + (j / 4) * 8 + hf * 4 + j % 4
   half8 one[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int j = 0; j < 8; ++j) one[c][j] = (_Float16)(16 * c + (j >> 2) * 8 + hf * 4 + (j & 3) == l32 ? 1.0f : 0.0f);
-  // plane h of 16 rows (chunk c) of a block
-  auto half_of = [&](const f32x16 &v, int c, int h) {
-    half8 o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const _Float16 hi = (_Float16)v[c * 8 + j];
-      o[j] = h == 0 ? hi : (_Float16)(v[c * 8 + j] - (float)hi);
-    }
-    return o;
-  };
   // rows r * 32 .. of a symmetric 64 x 64 plane pair as the first factor, chunk c of its columns in that order of k
   auto rows_of = [&](const _Float16 *p, int r, int c, int h) {
     const _Float16 *q = p + h * 4096;
@@ -502,12 +506,15 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
 #pragma unroll
         for (int h = 0; h < P; ++h) {
           f32x16 d = {};
-          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(x[b][r], 0, h), one[0], d, 0, 0, 0);
-          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(x[b][r], 1, h), one[1], d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x[b][r][0][h]), one[0], d, 0, 0, 0);
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x[b][r][1][h]), one[1], d, 0, 0, 0);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c) {  // (the values are f16 already: no rounding)
+            u32x4 w;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) xt[r][c][h][j] = (_Float16)d[c * 8 + j];
+            for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(d[c * 8 + 2 * j], d[c * 8 + 2 * j + 1]));
+            xt[r][c][h] = __builtin_bit_cast(half8, w);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -572,50 +579,53 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
     }
     __syncthreads();
     // X <- a X + B X
-    const float inv = 1.0f / sb;
-#pragma unroll
-    for (int b = 0; b < SMALL_NB; ++b)
-#pragma unroll
-      for (int r = 0; r < RB; ++r) asm volatile("" : "+v"(x[b][r]));  // (or the halves made for A are all kept until here)
+    const float inv = 1.0f / sb, out = 1.0f / sx;
+    const bool last = step + 1 == steps;
 #pragma unroll
     for (int b = 0; b < SMALL_NB; ++b) {
       if (b >= nb) continue;
-      half8 f[RB][2][P];
+      f32x16 d[RB] = {};
 #pragma unroll
       for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int h = 0; h < P; ++h) f[r][c][h] = half_of(x[b][r], c, h);
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        f32x16 d = {};
 #pragma unroll
         for (int c = 0; c < 2 * RB; ++c) {
           half8 p[P];
 #pragma unroll
           for (int h = 0; h < P; ++h) p[h] = rows_of(bm, r, c, h);
           if (P == 2) {
-            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], f[c >> 1][c & 1][0], d, 0, 0, 0);
-            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], f[c >> 1][c & 1][P - 1], d, 0, 0, 0);
+            d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][0]), d[r], 0, 0, 0);
+            d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][P - 1]), d[r], 0, 0, 0);
           }
-          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], f[c >> 1][c & 1][0], d, 0, 0, 0);
+          d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][0]), d[r], 0, 0, 0);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[b][r][e] = fmaf(ca, x[b][r][e], d[e] * inv);
+      for (int r = 0; r < RB; ++r) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          auto half_at = [&](int h) {
+            const uint32_t word = x[b][r][e >> 3][h][(e & 7) >> 1];  // (a bit cast of the vector's element itself reads element 0)
+            return (float)__builtin_bit_cast(half2_, word)[e & 1];
+          };
+          v[e] = fmaf(ca, P == 2 ? half_at(0) + half_at(P - 1) : half_at(0), d[r][e] * inv);
+        }
+        if (!last) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) keep(x[b][r], e, v[e], v[e + 1]);
+        } else {
+          int row4 = hf * 4, col = l32;
+          asm volatile("" : "+v"(row4), "+v"(col));  // (addresses made here, not kept through the steps)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = (wave + 8 * b) * 32 + col, i = r * 32 + (e >> 2) * 8 + row4 + (e & 3);
+            if (j < L && i < S) from_f32(v[e] * out, ((E *)m.out)[(uint32_t)(tall ? j * S + i : i * L + j)]);
+          }
+        }
+        packed(x[b][r]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  const float inv = 1.0f / sx;
-#pragma unroll
-  for (int b = 0; b < SMALL_NB; ++b)
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int j = (wave + 8 * b) * 32 + col, i = r * 32 + (e >> 2) * 8 + row4 + (e & 3);
-        if (b < nb && j < L && i < S) from_f32(x[b][r][e] * inv, ((E *)m.out)[(uint32_t)(tall ? j * S + i : i * L + j)]);
-      }
 }
 
 static bool is_small(int rows, int cols) {
