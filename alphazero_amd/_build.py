@@ -19,10 +19,9 @@ LIB = os.environ.get("AZ_ENGINE_LIB") or os.path.join(LIB_DIR, "libaz_engine.so"
 # -ffp-contract=off + correctly rounded f32 divide/sqrt: the PUCT / prior arithmetic must round exactly
 # like the reference's torch-CPU chain (bit-exactness notes).
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=off",
-         "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-int-to-void-pointer-cast"]
-# the operator files: no packed f32 arithmetic (some of its forms are not safe on this card)
-OPS_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-OPS_SRCS = ("az_sample.hip", "az_norm.hip", "az_ortho.hip")
+         "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-int-to-void-pointer-cast",
+         # no packed f32 arithmetic: some of its forms are not safe on this card (the host pass warns that it does not know the feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 OBJ_DIR = os.path.join(LIB_DIR, "obj")  # per-source objects (git-ignored): only what changed is recompiled
 
 
@@ -45,7 +44,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         objs.append(obj)
         newest = max(os.path.getmtime(f) for f in [src, *headers] if os.path.exists(f))
         if force or not os.path.exists(obj) or os.path.getmtime(obj) < newest:
-            cmd = [hipcc, *FLAGS, *(OPS_FLAGS if os.path.basename(src) in OPS_SRCS else []), "-c", "-o", obj, src]
+            cmd = [hipcc, *FLAGS, "-c", "-o", obj, src]
             if verbose:
                 print(" ".join(cmd))
             jobs.append((cmd, subprocess.Popen(cmd)))
