@@ -622,7 +622,8 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
     // prefix ends (a few rows in a hundred), the mass is summed exactly.
     constexpr double OFF = 0x1p-17;
     const float mf = score_of(kmax), scf = (float)st.sc;
-    const bool rough = !cut_k && !inf_row && scf < 1e30f;
+    // (a factor below 2^-120, of a temperature next to infinity, would meet infinite differences)
+    const bool rough = !cut_k && !inf_row && scf < 1e30f && scf > 0x1p-120f;
     double part = 0.0;
     row.walk([&](const uint32_t *k, int i, int) {
       uint32_t on = 0;
@@ -769,7 +770,7 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
 }
 
 // the kernel that holds a row of n scores
-template <class T> static void launch(const Args &a, int rows, hipStream_t s) {
+template <class T> static void launch_rows(const Args &a, int rows, hipStream_t s) {
   const dim3 four((rows + 3) / 4), one(rows);
   if (a.n <= 64) hipLaunchKernelGGL((k_sample_wave<T, 1>), four, dim3(256), 0, s, a, rows);
   else if (a.n <= 128) hipLaunchKernelGGL((k_sample_wave<T, 2>), four, dim3(256), 0, s, a, rows);
@@ -778,6 +779,24 @@ template <class T> static void launch(const Args &a, int rows, hipStream_t s) {
   else if (a.n <= 1024) hipLaunchKernelGGL((k_sample_wave<T, 16>), four, dim3(256), 0, s, a, rows);
   else if (a.n <= 8192) hipLaunchKernelGGL((k_sample_block<T, 256>), one, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_sample_block<T, 1024>), one, dim3(1024), 0, s, a);
+}
+
+// a launch holds fewer than 2^32 threads: 2^21 rows at a time
+template <class T> static void launch(Args a, int rows, hipStream_t s) {
+  for (constexpr int MOST = 1 << 21;;) {
+    const int m = rows < MOST ? rows : MOST;
+    launch_rows<T>(a, m, s);
+    if ((rows -= m) == 0) return;
+    a.scores = (const T *)a.scores + m * a.stride;
+    if (a.legal) a.legal += m * a.legal_stride;
+    a.u += m;
+    a.actions += m;
+    if (a.logp) a.logp += m;
+    if (a.t_rows) a.t_rows += m;
+    if (a.p_rows) a.p_rows += m;
+    if (a.mp_rows) a.mp_rows += m;
+    if (a.k_rows) a.k_rows += m;
+  }
 }
 
 }  // namespace azsample

@@ -215,3 +215,52 @@ def test_frequencies_follow_the_weights():
     n = torch.bincount(a.long().cpu(), minlength=7).double()
     assert n[0] == 0 and n[5] == 0
     assert bool(((n / rows - p).abs() <= 5 * (p * (1 - p) / rows).sqrt()).all())
+
+
+@pytest.mark.parametrize("n", [225, 5000])
+def test_temperatures_next_to_infinity(n):
+    """the weights of scores however far apart become alike; masked scores still weigh nothing"""
+    s, u = rand(8, n, torch.float32, 51)
+    s[1] *= 1e38
+    s[2, ::2] = 3e38
+    s[2, 1::2] = -3e38
+    s[3, ::3] = -math.inf
+    s[4] *= 1e-30
+    s[5, 0] = math.inf
+    legal = torch.rand(8, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(52)) < 0.5
+    for t in (math.inf, 1e300, 1e39, 1e37, 1e30):
+        check(s, u, t, 0, 0.5, 0.0, legal)
+        check(s, u, t, 0, 0.75)
+        check(s, u, t, 40, 0.5, 0.1, legal)
+
+
+@pytest.mark.parametrize("n", [5, 1100])
+def test_more_rows_than_one_launch_holds(n):
+    from alphazero_amd import ops
+
+    rows = (1 << 21) + 70
+    s, _ = rand(1, n, torch.float32, 53)
+    g = torch.Generator(device="cuda").manual_seed(54)
+    u = torch.rand(rows, device="cuda", generator=g)
+    k = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    k[-50:] = 1  # (the last launch reads its own rows' settings)
+    got, logp = ops.sample_actions(s.expand(rows, n), u, top_k=k, temperature=torch.ones(rows, device="cuda"), return_logprobs=True)
+    w = torch.exp((s[0].double() - s[0].max().double()))
+    mass = torch.cumsum(w, 0)
+    want = torch.searchsorted(mass, u.double() * mass[-1], right=True)
+    want[-50:] = s[0].argmax()
+    assert torch.equal(got.long(), want)
+    lp = (w / mass[-1]).log()[want]
+    lp[-50:] = 0.0
+    assert bool(((logp.double() - lp).abs() <= 2.0 ** -23 * (1 + lp.abs())).all())
+
+
+def test_rows_beyond_32_bit_offsets():
+    """rows 2^30 scores apart: the last one starts at byte 2^33"""
+    rows, far = 5, 1 << 30
+    s = torch.empty(rows * far, dtype=torch.bfloat16, device="cuda").view(rows, far)
+    on = torch.empty(rows * far, dtype=torch.bool, device="cuda").view(rows, far)
+    for n in (300, 5000):
+        v, u = rand(rows, n, torch.bfloat16, 55)
+        s[:, :n], on[:, :n] = v, torch.rand(rows, n, device="cuda") < 0.5
+        check(s[:, :n], u, 0.9, 0, 0.8, 0.0, on[:, :n])
