@@ -346,7 +346,7 @@ template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cols = a.cols, cgv = a.cg / V;
   const int64_t n = blockIdx.x / a.slices;
   const int col = (int)(blockIdx.x - n * a.slices) * cols + (tid & (cols - 1)), cv = a.c / V, p0 = tid / cols, step = NT / cols;
-  // the sample's bytes: a uniform base and a 32-bit offset (a resident sample has at most 4,096 pixels of 32 KiB).  Pixels behind the
+  // the sample's bytes: a uniform base and a 32-bit offset (a resident sample has at most 1,024 pixels of 64 KiB).  Pixels behind the
   // sample read its last one; their words are cleared before they count
   const int64_t base = n * a.hw * a.c * (int64_t)sizeof(T);
   const char *x = (const char *)a.x + base, *r = (const char *)a.r + base;
@@ -541,7 +541,8 @@ static int check(const char *&msg, int32_t dtype, int32_t param_dtype, int64_t n
   if (param_dtype != AZ_NN_F32 && param_dtype != dtype) { msg = "group norm: weight and bias are f32 or of x's dtype"; return AZ_EINVAL; }
   if (act != AZ_ACT_NONE && act != AZ_ACT_RELU && act != AZ_ACT_SILU) { msg = "group norm: unknown activation"; return AZ_EINVAL; }
   if (n < 0 || hw < 0 || c < 1 || c > MAX_C || g < 1 || g > MAX_G || c % g) { msg = "group norm: 1 <= C <= 16,384 a multiple of the groups, at most 1,024 groups"; return AZ_EINVAL; }
-  if (n > (1 << 28) || hw > (1 << 28) || n * g > 0x7FFFFFFF) { msg = "group norm: at most 2^28 samples of 2^28 pixels, 2^31 - 1 groups in all"; return AZ_EINVAL; }
+  // (a workgroup of 256 a group, and a launch holds fewer than 2^32 threads)
+  if (n >= (1 << 24) || hw > (1 << 28) || n * g >= (1 << 24)) { msg = "group norm: at most 2^24 - 1 groups in all samples, 2^28 pixels"; return AZ_EINVAL; }
   if (!(eps >= 0.0)) { msg = "group norm: eps >= 0"; return AZ_EINVAL; }
   return AZ_OK;
 }
@@ -642,7 +643,7 @@ int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t
   const int vec = vec_of(dtype, a.cg, ptrs, 3);
   int nv = 0;
   a.cols = cols_of(dtype, vec, c, a.cg, a.hw, 16, nv);
-  if (a.cols && n * (c / (16 / es) / a.cols) <= 0x7FFFFFFF) {
+  if (a.cols) {
     a.slices = c / (16 / es) / a.cols;
     return by_dtype(dtype, [&](auto t) {
       return by_count(nv, [&](auto k) {
@@ -708,7 +709,7 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
   const int vec = vec_of(dtype, a.cg, ptrs, 5);
   int nv = 0, rc;
   a.cols = cols_of(dtype, vec, c, a.cg, a.hw, 8, nv);
-  if (a.cols && n * (c / (16 / es) / a.cols) <= 0x7FFFFFFF) {
+  if (a.cols) {
     a.slices = c / (16 / es) / a.cols;
     rc = by_dtype(dtype, [&](auto t) {
       return by_count(nv, [&](auto k) {

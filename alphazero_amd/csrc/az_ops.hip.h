@@ -48,7 +48,7 @@ inline int launched(const char *what) noexcept {
 
 inline bool misaligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
 
-// 16-bit formats as raw bits: the widening is exact, the narrowing rounds to nearest even (half a step: 2^-9 of a bf16, 2^-12 of an f16)
+// 16-bit formats as raw bits: the widening is exact, the narrowing rounds to nearest even (half a step: at most 2^-8 of a bf16's value, 2^-11 of an f16's)
 struct bf16_t { uint16_t b; };
 struct f16_t { _Float16 h; };
 

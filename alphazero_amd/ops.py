@@ -90,7 +90,7 @@ def sample_actions(scores: torch.Tensor, uniforms: torch.Tensor, *, temperature=
     k_t, k_v = _per_row(top_k, "top_k", rows, torch.int32, dev)
     p_t, p_v = _per_row(top_p, "top_p", rows, torch.float32, dev)
     m_t, m_v = _per_row(min_p, "min_p", rows, torch.float32, dev)
-    if not (t_v >= 0 and k_v >= 0 and p_v >= 0 and 0 <= m_v <= 1) or k_v != int(k_v):
+    if not (t_v >= 0 and 0 <= k_v < float("inf") and p_v >= 0 and 0 <= m_v <= 1) or k_v != int(k_v):
         raise EngineError("temperature >= 0, top_k >= 0 (a whole number), top_p >= 0 and 0 <= min_p <= 1")
     with _on(dev):
         actions = torch.empty(rows, dtype=torch.int32, device=dev)
@@ -178,8 +178,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise EngineError(f"activation: one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     if not isinstance(num_groups, int) or num_groups < 1 or c < 1 or c % num_groups or c > 16384 or num_groups > 1024:
         raise EngineError(f"{c} channels in {num_groups} groups: expected 1 .. 16,384 channels, a multiple of 1 .. 1,024 groups")
-    if n > 1 << 28 or h * w > 1 << 28 or n * num_groups >= 1 << 31:
-        raise EngineError("at most 2^28 samples of 2^28 pixels, 2^31 - 1 groups in all")
+    if h * w > 1 << 28 or n * num_groups >= 1 << 24:
+        raise EngineError("at most 2^24 - 1 groups in all samples, 2^28 pixels a sample")
     if not eps >= 0.0:
         raise EngineError("eps >= 0")
     dtypes = {x.dtype, torch.float32}

@@ -472,8 +472,8 @@ int az_sample_actions(int32_t dtype, int32_t rows, int32_t n, const void *scores
  * Backward: dy_dev like x; dx_dev, dresidual_dev like x, dweight_dev, dbias_dev (c) of param_dtype, each may be NULL (not wanted).
  *   relu's derivative at 0 is 0.  n * hw = 0: nothing is written but zero dweight / dbias.
  * workspace_dev: az_group_norm_workspace() bytes (backward 0 / 1; -1: refused), aligned to 16 bytes, meaningless between calls; calls that
- * overlap in time need one each.  c at most 16,384, at most 1,024 groups, 2^28 samples, 2^28 pixels, n * groups below 2^31.  No output may overlap an input
- * or another output.  The result does not depend on timing: sums are taken in a fixed order. */
+ * overlap in time need one each.  c at most 16,384, at most 1,024 groups, 2^28 pixels, n * groups below 2^24.  No output may
+ * overlap an input or another output.  The result does not depend on timing: sums are taken in a fixed order. */
 int64_t az_group_norm_workspace(int32_t backward, int64_t n, int64_t hw, int32_t c, int32_t groups);
 int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t hw, int32_t c, int32_t groups, int32_t act, double eps,
                           const void *x_dev, const void *residual_dev, const void *weight_dev, const void *bias_dev, void *y_dev,
@@ -487,7 +487,7 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
  * Adam: training/nn_trainer.py:36-94):
  *   X = M / (|M|_F + eps), on the shorter side;  `steps` times:  A = X X^T,  X = a X + (b A + c A^2) X;  out = X
  * in / out: HOST arrays of `count` device pointers, row-major dense matrices of `dtype` with rows[i] x cols[i] elements (a side of 0:
- * nothing to do; at most 65,536); out[i] may be in[i].  f32 and f16 matrices are computed to f32 accuracy (each factor in two f16
+ * nothing to do; at most 65,536); out[i] may be in[i], and otherwise overlaps no matrix of the call.  f32 and f16 matrices are computed to f32 accuracy (each factor in two f16
  * halves), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
  * under which a singular value in [0, 1] could grow beyond 7.5 are refused.
  * workspace_dev: az_orthogonalize_workspace() bytes (-1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in

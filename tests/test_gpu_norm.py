@@ -321,3 +321,41 @@ def test_self_play_on_a_group_norm_net():
     eng.check()
     assert bool((acts >= 0).all()) and bool((acts < 81).all())
     eng.close()
+
+
+@pytest.mark.parametrize("shape", [(1900000, 128, 3, 3, 8), (9, 64, 2048, 2048, 8)], ids=lambda s: "x".join(map(str, s)))
+def test_more_than_2_31_elements(shape):
+    """the last samples, whose offsets pass 32 bits, forward and backward; the parameters' gradients in f64 sums over shares of the batch"""
+    from alphazero_amd import ops
+
+    n, c, h, w, g = shape
+    base = torch.randn(4096 * 9 * 128 + 1, device="cuda", generator=torch.Generator(device="cuda").manual_seed(61)).bfloat16()
+    total = n * c * h * w
+    x, dy = (torch.empty(total, dtype=torch.bfloat16, device="cuda").view(n, h, w, c).permute(0, 3, 1, 2) for _ in range(2))
+    for t, shift in ((x, 0), (dy, 1000)):  # (the numbers repeat, out of step with the samples)
+        flat, m = t.permute(0, 2, 3, 1).reshape(-1), base.numel()
+        reps = total // m
+        flat[:reps * m].view(reps, m).copy_(base.roll(shift).expand(reps, m))
+        flat[reps * m:] = base[:total - reps * m]
+    wt, b = torch.linspace(0.5, 1.5, c, device="cuda").requires_grad_(True), torch.linspace(-0.3, 0.3, c, device="cuda").requires_grad_(True)
+    x.requires_grad_(True)
+    y = ops.group_norm_act(x, g, wt, b, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, [x, wt, b], dy)
+    k = max(1, min(n, (1 << 28) // (c * h * w)))
+    sw, sb, mw, mb = (torch.zeros(c, dtype=torch.float64, device="cuda") for _ in range(4))
+    for lo in range(0, n, k):
+        ts = [t.detach()[lo:lo + k].double() if t.dim() == 4 else t.detach().double() for t in (x, wt, b)]
+        for t in ts:
+            t.requires_grad_(True)
+        d = dy[lo:lo + k].double()
+        ref = plain(ts[0], g, ts[1], ts[2], None, 1e-5, "relu")
+        rdx, rdw, rdb = torch.autograd.grad(ref, ts, d)
+        sw += rdw
+        sb += rdb
+        with torch.no_grad():
+            mw += (d.abs() * plain(ts[0], g, torch.ones_like(ts[1]), None, None, 1e-5, "none").abs()).sum((0, 2, 3))
+            mb += d.abs().sum((0, 2, 3))
+            assert bool(((y[lo:lo + k].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -15).all())
+            assert bool(((dx[lo:lo + k].double() - rdx).abs() <= 2.0 ** -8 * rdx.abs() + 2.0 ** -13).all())
+        del ts, d, ref, rdx
+    assert bool(((dw.double() - sw).abs() <= 2.0 ** -16 * mw).all()) and bool(((db.double() - sb).abs() <= 2.0 ** -16 * mb).all())

@@ -190,3 +190,14 @@ def test_muon_steps():
     opt2 = Muon(ps + [frozen], lr=0.5)
     opt2.load_state_dict(state)
     assert opt2.param_groups[0]["lr"] == 0.02 and torch.equal(opt2.state[ps[0]]["momentum"], opt.state[ps[0]]["momentum"])
+
+
+def test_workspace_beyond_32_bit_offsets():
+    """the second matrix's buffers start past 4 GiB of the workspace; a matrix's result is the same there, bit for bit"""
+    from alphazero_amd import ops
+
+    m = torch.randn(4096, 65536, device="cuda", generator=torch.Generator(device="cuda").manual_seed(71))
+    one = ops.orthogonalize(m, steps=2)
+    two = ops.orthogonalize([m, m], steps=2)
+    assert torch.equal(two[0], one) and torch.equal(two[1], one)
+    check(m, one, steps=2)

@@ -59,7 +59,7 @@ def test_sample_python_refusals_on_the_gpu():
                 lambda: ops.sample_actions(s[:, :0], u), lambda: ops.sample_actions(s, u, legal=torch.ones(2, 9, device="cuda")),
                 lambda: ops.sample_actions(s, u, legal=torch.ones(2, 8, device="cuda", dtype=torch.bool)),
                 lambda: ops.sample_actions(s, u, temperature=-1.0), lambda: ops.sample_actions(s, u, temperature=float("nan")),
-                lambda: ops.sample_actions(s, u, top_k=1.5), lambda: ops.sample_actions(s, u, top_k=-1), lambda: ops.sample_actions(s, u, min_p=1.1),
+                lambda: ops.sample_actions(s, u, top_k=1.5), lambda: ops.sample_actions(s, u, top_k=float("inf")), lambda: ops.sample_actions(s, u, top_k=-1), lambda: ops.sample_actions(s, u, min_p=1.1),
                 lambda: ops.sample_actions(s, u, top_p=torch.ones(3, device="cuda")), lambda: ops.sample_actions(s, u, top_k=torch.ones(2, device="cuda"))):
         with pytest.raises(EngineError):
             bad()
@@ -83,6 +83,15 @@ def test_norm_refuses(bad, backward):
     lib = _lib()
     assert _norm(lib, backward, **bad) == -1
     assert lib.az_tower_last_error().startswith(b"group norm:")
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_norm_refuses_more_workgroups_than_a_launch_holds(backward):
+    lib = _lib()
+    for n, c, g in ((1 << 24, 1, 1), (1 << 21, 8, 8), ((1 << 14), 1024, 1024)):
+        assert _norm(lib, backward, n=n, c=c, g=g, hw=1, size=1 << 60) == -1
+        assert b"2^24" in lib.az_tower_last_error()
+        assert lib.az_group_norm_workspace(int(backward), n, 1, c, g) == -1
 
 
 def test_norm_sizes():
