@@ -7,6 +7,7 @@ HIP graph.  There is no CPU path: a tensor elsewhere, or a shape or type a kerne
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -18,15 +19,19 @@ def _check(rc: int) -> None:
         raise EngineError(f"az call failed ({rc}): {load_library().az_tower_last_error().decode()}")
 
 
+# (the stream and the device without the Python objects around them: 8 us less a call in autograd's thread)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _stream(device: torch.device) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return C.c_void_p(_raw_stream(device.index))
 
 
 class _on:
     """the device current for the allocations inside, without a switch where it is current already"""
 
     def __init__(self, device: torch.device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if _current_device() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
@@ -111,15 +116,15 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 
 def _empty_like(x: torch.Tensor) -> torch.Tensor:
-    n, c, h, w = x.shape
-    return torch.empty((n, h, w, c), dtype=x.dtype, device=x.device).permute(0, 3, 1, 2)
+    return torch.empty_like(x, memory_format=torch.channels_last)
 
 
-def _workspace(backward: int, n: int, hw: int, c: int, groups: int, device) -> torch.Tensor:
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(backward: int, n: int, hw: int, c: int, groups: int) -> int:
     size = load_library().az_group_norm_workspace(backward, n, hw, c, groups)
     if size < 0:
         _check(-1)
-    return torch.empty(max(int(size), 16), dtype=torch.uint8, device=device)
+    return max(int(size), 16)
 
 
 class _GroupNormAct(torch.autograd.Function):
@@ -133,11 +138,12 @@ class _GroupNormAct(torch.autograd.Function):
         pd = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         with _on(x.device):
             y = _empty_like(x)
-            stats = torch.empty((n, groups, 2), dtype=torch.float64, device=x.device)
-            ws = _workspace(0, n, h * w, c, groups, x.device)
+            size = _norm_workspace(0, n, h * w, c, groups)
+            stats = torch.empty(n * groups * 2 + size // 8, dtype=torch.float64, device=x.device)  # the workspace behind the statistics
+            ws = stats.data_ptr() + n * groups * 16
             _check(load_library().az_group_norm_forward(
                 _NN_DTYPES[x.dtype], _NN_DTYPES[pd], n, h * w, c, groups, act, float(eps), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias),
-                _ptr(y), _ptr(stats), _ptr(ws), ws.numel(), _stream(x.device)))
+                _ptr(y), _ptr(stats), ws, size, _stream(x.device)))
         ctx.save_for_backward(x, weight, bias, residual, stats)
         ctx.groups, ctx.act, ctx.pd = groups, act, pd
         return y
@@ -154,11 +160,12 @@ class _GroupNormAct(torch.autograd.Function):
             dw = torch.empty(c, dtype=ctx.pd, device=x.device) if need_w else None
             db = torch.empty(c, dtype=ctx.pd, device=x.device) if need_b else None
             dr = _empty_like(x) if need_r and ctx.act else None
-            ws = _workspace(1, n, h * w, c, ctx.groups, x.device)
+            size = _norm_workspace(1, n, h * w, c, ctx.groups)
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
             if need_x or need_w or need_b or dr is not None:
                 _check(load_library().az_group_norm_backward(
                     _NN_DTYPES[x.dtype], _NN_DTYPES[ctx.pd], n, h * w, c, ctx.groups, ctx.act, _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias),
-                    _ptr(dy), _ptr(stats), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream(x.device)))
+                    _ptr(dy), _ptr(stats), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), size, _stream(x.device)))
         if need_r and dr is None:
             dr = dy  # (no activation: the sum passes the gradient on)
         return dx, dw, db, dr, None, None, None
