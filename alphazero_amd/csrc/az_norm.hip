@@ -47,6 +47,20 @@ template <class T, int V> __device__ __forceinline__ void store(T *p, const floa
 template <class T> __device__ __forceinline__ float param(const void *p, int f32, int i, float none) {
   return p == nullptr ? none : f32 ? ((const float *)p)[i] : to_f32(((const T *)p)[i]);
 }
+// V neighbouring ones at once (the pointer is aligned to its elements only)
+template <class T, int V> __device__ __forceinline__ void params(const void *p, int f32, int i, float none, float *o) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = none;
+  } else if (f32) {
+    __builtin_memcpy(o, (const float *)p + i, V * 4);
+  } else {
+    T t[V];
+    __builtin_memcpy(t, (const T *)p + i, sizeof(t));
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = to_f32(t[j]);
+  }
+}
 template <class T> __device__ __forceinline__ void put_param(void *p, int f32, int i, double v) {
   if (p == nullptr) return;
   if (f32) ((float *)p)[i] = (float)v;
@@ -175,6 +189,7 @@ __global__ __launch_bounds__(NT) void k_gn_stats_join(Args a) {
   const int g = (int)(ng - n * a.g), lane = threadIdx.x & 63;
   if (n >= a.n) return;
   double s = 0.0, q = 0.0;
+#pragma unroll 4
   for (int i = lane; i < a.chunks; i += 64) { const double *p = a.part + ((n * a.chunks + i) * a.g + g) * 2; s += p[0]; q += p[1]; }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
@@ -192,8 +207,8 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_apply(Args 
     const double *sd = a.stats + (n * a.g + col * V / a.cg) * 2;
     const Stat s = stat_of(sd[0], sd[1]);
     float w[V], b[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+    params<T, V>(a.w, a.param_f32, col * V, 1.0f, w);
+    params<T, V>(a.b, a.param_f32, col * V, 0.0f, b);
 #pragma unroll 2
     for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
       const int64_t at = base + (int64_t)p * a.c + col * V;
@@ -222,8 +237,8 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_sums(Ar
       const double sd2[2] = {sd[0], sd[1]};
       const Stat st = stat_of(sd2[0], sd2[1]);
       float w[V], b[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+      params<T, V>(a.w, a.param_f32, col * V, 1.0f, w);
+      params<T, V>(a.b, a.param_f32, col * V, 0.0f, b);
 #pragma unroll 2
       for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
         const int64_t at = base + (int64_t)p * a.c + col * V;
@@ -266,6 +281,7 @@ template <class T> __global__ __launch_bounds__(NT) void k_gn_bwd_join(Args a) {
     const int c = g * a.cg + c0 + tx;
     double s = 0.0, q = 0.0;
     if (c0 + tx < a.cg && ty < ty_n)
+#pragma unroll 8
       for (int i = ty; i < a.chunks; i += ty_n) { const float *p = a.cpart + ((n * a.chunks + i) * a.c + c) * 2; s += p[0]; q += p[1]; }
     s_[tid] = s;
     q_[tid] = q;
@@ -304,8 +320,8 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_bwd_dx(Args
     const Stat st = stat_of(sd2[0], sd2[1]);
     const float m1 = a.gsum[(n * a.g + g) * 2], m2 = a.gsum[(n * a.g + g) * 2 + 1];
     float w[V], b[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) { w[j] = param<T>(a.w, a.param_f32, col * V + j, 1.0f); b[j] = param<T>(a.b, a.param_f32, col * V + j, 0.0f); }
+    params<T, V>(a.w, a.param_f32, col * V, 1.0f, w);
+    params<T, V>(a.b, a.param_f32, col * V, 0.0f, b);
 #pragma unroll 2
     for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
       const int64_t at = base + (int64_t)p * a.c + col * V;
