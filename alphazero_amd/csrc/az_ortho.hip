@@ -38,11 +38,11 @@ struct Mat {
   int32_t rows, cols;
 };
 enum { GRAM, POLY, UPDATE, LAST };  // (POLY has GRAM's tiles, LAST has UPDATE's)
-enum { WHOLE, PART, JOIN };  // a tile's product at once; a share of its k range; the shares' sum and what follows a product
+enum { WHOLE, SPLIT, JOIN };  // a tile's product at once; that, or for tiles from `whole` on a share of its k range; the shares' sum and what follows a product
 struct Table {  // what the first launch carries and leaves at the start of the workspace for the others
   Mat m[MAX_M];
-  uint32_t start[4][MAX_M];  // first tile of each matrix: of A and B, of X, of PACK; first partial tile of A
-  int32_t shares[MAX_M];     // of A's k range
+  uint32_t start[6][MAX_M];  // first tile of each matrix: of A and B, of X, of PACK; share of a cut tile; cut tile; tile done at once
+  int32_t shares[MAX_M];     // of a cut tile's k range
   int32_t count;
 };
 struct Args {
@@ -51,7 +51,7 @@ struct Args {
   float sx, sa, sb;  // powers of two: the stored X, A and B are sx, sa and sb times theirs
   double eps;
   int32_t count, cur;
-  int32_t n[4];     // tiles in all, as in Table::start
+  int32_t n[6];     // tiles in all, as in Table::start
   uint64_t part;    // byte offset of the partial tiles
 };
 
@@ -129,11 +129,11 @@ template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char
 
 // Workgroups go round the 8 XCDs in turn; block b takes item (b % 8) * ceil(n / 8) + b / 8 of n, so that an XCD (and its L2) gets a
 // run of neighbouring tiles, and much the same matrices in every phase.  -> -1: none (the grid is rounded up to whole turns)
-__device__ __forceinline__ int item_of(int n) {
-  const int per = (n + 7) / 8, t = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  return (int)(blockIdx.x >> 3) < per && t < n ? t : -1;
+__device__ __forceinline__ int item_of(int n, int block) {
+  const int per = (n + 7) / 8, t = (block & 7) * per + (block >> 3);
+  return (block >> 3) < per && t < n ? t : -1;
 }
-static unsigned grid_of(uint32_t n) { return (n + 7) / 8 * 8; }
+__host__ __device__ static inline unsigned grid_of(uint32_t n) { return (n + 7) / 8 * 8; }
 
 // tile -> (matrix, tile of it): the lanes look at one matrix's first tile each
 __device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
@@ -150,7 +150,7 @@ __device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
 template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_pack(Args a, int parts) {
   __shared__ float t_[64][65];
   __shared__ double s_[NT / 64];
-  int tile = item_of(a.n[2]);
+  int tile = item_of(a.n[2], blockIdx.x);
   if (tile < 0) return;
   const int tid = threadIdx.x, mi = find(a, 2, tile);
   const Mat m = ((const Table *)a.ws)->m[mi];
@@ -223,25 +223,48 @@ template <int PHASE> __host__ __device__ __forceinline__ int tiles_of(const Lay 
   return PHASE == GRAM || PHASE == POLY ? s * (s + 1) / 2 : s * l;
 }
 
+// Which of A's tiles are cut along k, by the matrix alone (its result must not depend on the others in the call): those from `whole` on, in
+// `shares` each.
+//   tiles of 64: at most 96 of them leave CUs idle, and with 32 stages or more a share of 8 stages or more is worth the second pass; A only.
+//   tiles of 128: two workgroups a CU hold 512 at a time (one plane), one 256 (two planes); what little is left over after whole turns would
+//   take a turn of its own.  B = A A as well (its k range is the short side, 28 stages or more).  4096 x 4096 bf16, 528 tiles: 112 us at once,
+//   97 with the last 16 in four shares each (102 in two, 105 in sixteen: those wait for the join).
+struct Split { int whole, shares; };
+__host__ __device__ __forceinline__ Split split_of(const Lay &y, int tile) {
+  const int tiles = tiles_of<GRAM>(y, tile);
+  if (tile == 64) {
+    const int stages = y.lp * 2 * y.planes / UNIT;
+    if (tiles > 96 || stages < 32) return Split{tiles, 1};
+    const int s = 512 / tiles < stages / 8 ? 512 / tiles : stages / 8;
+    return Split{s > 1 ? 0 : tiles, s < 8 ? s : 8};
+  }
+  const int turn = y.planes == 1 ? 512 : 256, left = tiles % turn;
+  if (tiles < turn || left == 0 || left > turn / 4) return Split{tiles, 1};
+  return Split{tiles - left, 4};
+}
+
 // One T x T tile, four waves, (T / 2) x (T / 2) each in blocks of 32 x 32.  T = 64, and T = 128 with two planes, which leaves a CU one
 // workgroup: four stages in LDS, the moves of three under way while one is multiplied.  T = 128 with one plane: two stages, and two
 // workgroups a CU cover for each other.
-// A long A with few tiles is cut along k (PART): every share leaves its sums as they lie in its registers, and JOIN adds the shares in
+// Tiles of A (and of B) may be cut along k (split_of): every share leaves its sums as they lie in its registers, and JOIN adds the shares in
 // order and goes on as WHOLE does.
 template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds__(NT) void k_os_gemm(Args a) {
   constexpr bool SYM = PHASE == GRAM || PHASE == POLY;
   constexpr int B = T / 64, W = T / 2, STAGE = 2 * T * UNIT, BUFS = T == 64 || P == 2 ? 4 : 2, MOVES = 2 * T / 8 / 4;
   __shared__ __attribute__((aligned(1024))) char lds[BUFS * STAGE];
-  constexpr int KIND = MODE == PART ? 3 : SYM ? 0 : 1;
-  int tile = item_of(a.n[KIND]);
+  // SPLIT: the tiles done at once, then the shares of the others (shorter, they fill what the last of those leave idle)
+  const int ahead = MODE == SPLIT ? (int)grid_of(a.n[5]) : 0;
+  const bool part = MODE == SPLIT && (int)blockIdx.x >= ahead;
+  const int kind = MODE == SPLIT ? (part ? 3 : 5) : MODE == JOIN ? 4 : SYM ? 0 : 1;
+  int tile = item_of(a.n[kind], part ? blockIdx.x - ahead : blockIdx.x);
   if (tile < 0) return;
-  const int mi = find(a, KIND, tile);
-  const int shares = MODE == WHOLE ? 1 : ((const Table *)a.ws)->shares[mi], share = MODE == PART ? tile % shares : 0;
-  if (MODE == PART) tile /= shares;
-  const int64_t first = MODE == WHOLE ? 0 : (int64_t)((const Table *)a.ws)->start[3][mi] + (int64_t)tile * shares + share;  // partial tile
+  const int mi = find(a, kind, tile);
+  const int shares = MODE == JOIN || part ? ((const Table *)a.ws)->shares[mi] : 1, share = part ? tile % shares : 0;
+  const int64_t first = MODE == WHOLE ? 0 : (int64_t)((const Table *)a.ws)->start[3][mi] + (int64_t)tile * (part ? 1 : shares);  // its sums
   const Mat m = ((const Table *)a.ws)->m[mi];
   const Lay y(m.rows, m.cols, P, T);
   char *ws = a.ws + m.ws;
+  if (MODE == JOIN || part) tile = split_of(y, T).whole + tile / (part ? shares : 1);
   int ti, tj;
   if (SYM) upper(tile, y.sp / T, ti, tj);
   else square(tile, y.sp / T, y.lp / T, ti, tj);
@@ -267,7 +290,7 @@ template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds
   f32x16 acc[B][B] = {}, low[P == 2 ? B : 1][P == 2 ? B : 1] = {};  // hi hi; hi lo + lo hi, joined at the end: a third of the roundings
   const int rp = (wi + (lane & 31)) * UNIT, rq = (T + wj + (lane & 31)) * UNIT, sw = lane & 7, hf = lane >> 5;
   if constexpr (MODE != JOIN) {
-  const int s0 = MODE == PART ? (int)((int64_t)stages * share / shares) : 0, s1 = MODE == PART ? (int)((int64_t)stages * (share + 1) / shares) : stages;
+  const int s0 = part ? (int)((int64_t)stages * share / shares) : 0, s1 = part ? (int)((int64_t)stages * (share + 1) / shares) : stages;
 #pragma unroll
   for (int s = 0; s < BUFS - 1; ++s)
     if (s0 + s < s1) issue(s0 + s);
@@ -303,24 +326,24 @@ template <int PHASE, int P, int T, class E, int MODE> __global__ __launch_bounds
   }
   stage_barrier<0>();
   }
-  if constexpr (MODE != WHOLE) {
+  if (MODE == JOIN || part) {
     // [tile][share][block][element][thread] f32
     constexpr int64_t STEP = (int64_t)B * B * 16 * NT;
-    float *part = (float *)(a.ws + a.part) + first * STEP + tid;
-    for (int k = 0; k < (MODE == PART ? 1 : shares); ++k) {
+    float *sums = (float *)(a.ws + a.part) + first * STEP + tid;
+    for (int k = 0; k < (MODE == JOIN ? shares : 1); ++k) {
 #pragma unroll
       for (int x = 0; x < B; ++x)
 #pragma unroll
         for (int z = 0; z < B; ++z)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float *q_ = part + ((x * B + z) * 16 + e) * NT;
-            if (MODE == PART) *q_ = P == 2 ? acc[x][z][e] + low[x][z][e] : acc[x][z][e];
-            else acc[x][z][e] += *q_;
+            float *q_ = sums + ((x * B + z) * 16 + e) * NT;
+            if (MODE == JOIN) acc[x][z][e] += *q_;
+            else *q_ = P == 2 ? acc[x][z][e] + low[x][z][e] : acc[x][z][e];
           }
-      part += STEP;
+      sums += STEP;
     }
-    if (MODE == PART) return;
+    if (MODE != JOIN) return;
   }
   // The results go through LDS, 32 rows of a wave's share at a time (a wave uses its own strip only), so that memory sees whole units:
   // first row by row, where the term a X or b A is added, then column by column for the mirror image or the transpose.
@@ -644,15 +667,6 @@ static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }
 // 0.53 / 1.34 and 0.34 / 0.59
 static int tile_of(int rows, int cols) { return (rows < cols ? rows : cols) >= 1792 ? 128 : 64; }
 
-// Shares of A's k range, by the matrix alone (a matrix's result must not depend on the others in the call): at most 96 tiles of 64 x 64
-// leave CUs idle, and with 32 stages or more a share of 8 stages or more is worth the second pass.
-static int shares_of(const Lay &y, int tile) {
-  const int tiles = tiles_of<GRAM>(y, tile), stages = y.lp * 2 * y.planes / UNIT;
-  if (tile != 64 || tiles > 96 || stages < 32) return 1;
-  const int s = 512 / tiles < stages / 8 ? 512 / tiles : stages / 8;
-  return s < 8 ? s : 8;
-}
-
 // One workgroup a matrix where every matrix of the call is small; beside larger ones they cost nothing in the others' launches, and a
 // launch of their own would (64 x 576 alone: 88 us in 17 launches, see above for one).
 static bool all_small(int count, const int32_t *rows, const int32_t *cols) {
@@ -697,8 +711,7 @@ static bool bounded(int steps, double a, double b, double c, Args &g) {
 struct Run {
   Table t;
   int tile;
-  bool shared;  // some A is cut
-  uint32_t n[4];
+  uint32_t n[6];
   uint64_t part, bytes;
 };
 
@@ -714,21 +727,21 @@ template <class F> static int each_run(int planes, int count, const void *const 
       if (r.t.count == 0 || (r.t.count < MAX_M && i < count - 1)) continue;
       uint64_t off = round_up(sizeof(Table));
       r.tile = tile;
-      r.shared = false;
       for (uint32_t &v : r.n) v = 0;
       for (int k = 0; k < r.t.count; ++k) {
         Mat &m = r.t.m[k];
         const Lay y(m.rows, m.cols, planes, tile);
         m.ws = off;
         off += (uint64_t)round_up(y.bytes());
-        const int shares = shares_of(y, tile), sym = tiles_of<GRAM>(y, tile);
-        r.t.shares[k] = shares;
-        r.shared |= shares > 1;
-        const uint32_t add[4] = {(uint32_t)sym, (uint32_t)tiles_of<UPDATE>(y, tile), (uint32_t)(y.sp / 64) * (uint32_t)(y.lp / 64), (uint32_t)(sym * shares)};
-        for (int q = 0; q < 4; ++q) { r.t.start[q][k] = r.n[q]; r.n[q] += add[q]; }
+        const Split split = split_of(y, tile);
+        const int sym = tiles_of<GRAM>(y, tile), cut = sym - split.whole;
+        r.t.shares[k] = split.shares;
+        const uint32_t add[6] = {(uint32_t)sym, (uint32_t)tiles_of<UPDATE>(y, tile), (uint32_t)(y.sp / 64) * (uint32_t)(y.lp / 64),
+                                 (uint32_t)(cut * split.shares), (uint32_t)cut, (uint32_t)split.whole};
+        for (int q = 0; q < 6; ++q) { r.t.start[q][k] = r.n[q]; r.n[q] += add[q]; }
       }
       r.part = off;
-      if (r.shared) off += (uint64_t)r.n[3] * tile * tile * 4;
+      off += (uint64_t)r.n[3] * tile * tile * 4;
       r.bytes = off;
       const int rc = f(r);
       if (rc != AZ_OK) return rc;
@@ -765,21 +778,26 @@ template <class E, int P, int T> static int run(const Run &r, Args a, int steps,
   const int parts = (int)(want < 1 ? 1 : want < NORM_PARTS ? want : NORM_PARTS);
   a.count = r.t.count;
   a.part = r.part;
-  for (int k = 0; k < 4; ++k) a.n[k] = (int)r.n[k];
-  const dim3 sym(grid_of(r.n[0])), all(grid_of(r.n[1]));
+  for (int k = 0; k < 6; ++k) a.n[k] = (int)r.n[k];
+  const dim3 sym(grid_of(r.n[0])), all(grid_of(r.n[1])), split(grid_of(r.n[5]) + grid_of(r.n[3])), join(grid_of(r.n[4]));
   hipLaunchKernelGGL((k_os_norm<E>), dim3(parts, r.t.count), dim3(NT), 0, s, r.t, a.ws);
   hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(grid_of(r.n[2])), dim3(NT), 0, s, a, parts);
   for (int k = 0; k < steps; ++k) {
     a.cur = k & 1;
-    if (r.shared) {
-      if constexpr (T == 64) {
-        hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, PART>), dim3(grid_of(r.n[3])), dim3(NT), 0, s, a);
-        hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, JOIN>), sym, dim3(NT), 0, s, a);
-      }
+    if (r.n[3]) {
+      hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, SPLIT>), split, dim3(NT), 0, s, a);
+      hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, JOIN>), join, dim3(NT), 0, s, a);
     } else {
       hipLaunchKernelGGL((k_os_gemm<GRAM, P, T, E, WHOLE>), sym, dim3(NT), 0, s, a);
     }
-    hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E, WHOLE>), sym, dim3(NT), 0, s, a);
+    if (T == 128 && r.n[3]) {
+      if constexpr (T == 128) {
+        hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E, SPLIT>), split, dim3(NT), 0, s, a);
+        hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E, JOIN>), join, dim3(NT), 0, s, a);
+      }
+    } else {
+      hipLaunchKernelGGL((k_os_gemm<POLY, P, T, E, WHOLE>), sym, dim3(NT), 0, s, a);
+    }
     if (k + 1 < steps) hipLaunchKernelGGL((k_os_gemm<UPDATE, P, T, E, WHOLE>), all, dim3(NT), 0, s, a);
     else hipLaunchKernelGGL((k_os_gemm<LAST, P, T, E, WHOLE>), all, dim3(NT), 0, s, a);
   }

@@ -201,3 +201,18 @@ def test_workspace_beyond_32_bit_offsets():
     two = ops.orthogonalize([m, m], steps=2)
     assert torch.equal(two[0], one) and torch.equal(two[1], one)
     check(m, one, steps=2)
+
+
+@pytest.mark.parametrize("shape,dtype", [((2900, 2950), torch.float32), ((2990, 2890), torch.float16), ((4090, 4150), torch.bfloat16), ((2000, 2500), torch.bfloat16)],
+                         ids=lambda v: str(v))
+def test_large_matrices_of_which_a_few_tiles_are_cut(shape, dtype):
+    """23 x 23 tiles of 128 leave 20 after a whole turn of 256, 32 x 32 leave 16 after one of 512"""
+    from alphazero_amd import ops
+
+    m = make(shape, dtype, 81)
+    one = ops.orthogonalize(m)
+    check(m, one)
+    other = make((300, 200), dtype, 82)
+    two = ops.orthogonalize([other, m, m])
+    assert torch.equal(two[1], one) and torch.equal(two[2], one)
+    check(other, two[0])
