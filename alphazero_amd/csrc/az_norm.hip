@@ -5,7 +5,14 @@
 //   dz = dy act'(z);  dr = dz;  dw = sum dz xhat;  db = sum dz;
 //   dx = rstd (dz w - mean_g(dz w) - xhat mean_g(dz w xhat))
 //
-// Bound by bytes: forward reads x (and r) and writes y, backward reads x, dy (and r) and writes dx (and dr).
+// Bound by bytes: forward reads x (and r) and writes y, backward reads x, dy (and r) and writes dx (and dr).  A large copy reaches 5.04 TB/s
+// on this card (reads and writes counted).  A sample whose channels fit a workgroup's registers is read once (k_gn_fwd_one, k_gn_bwd_one);
+// a larger one is shared out over workgroups and read twice.  Measured:
+//   1,024 x 128 x 15 x 15 f32, relu, residual: forward 76.7 us (354 MB: 4.6 TB/s), backward 117.8 us (590 MB: 5.0 TB/s) + 5.5 us for dw, db
+//   16,384 x 64 x 15 x 15 bf16, relu, forward: 162 us (944 MB: 5.8 TB/s)
+//   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.4 + 4.0 + 23.4 us, backward 26.4 + 4.9 + 33.4 + 4.2 us (66.6 MB a tensor: 3.3 TB/s over
+//                                              what the passes move; bound by instructions as much, 10 k a SIMD of 4 cycles in backward's)
+//   64 x 64 x 9 x 9 f32, relu:                 4.2 us, 4.7 + 3.0 us; the call is bound by the host (112 us with autograd's own 72)
 // Mean and variance come from f64 sums of x and x^2 (the products of two f32 are exact in f64, so one pass is enough even where
 // |mean| is 10^5 standard deviations); the mean is kept as a pair of f32 for the subtraction, everything per element is f32, and
 // each output is rounded once.  A relu's gradient hangs on the sign of z: where f32 cannot tell it, z is recomputed in f64.
@@ -537,8 +544,8 @@ template <class T, bool LAST> __global__ __launch_bounds__(WB_NT) void k_gn_wb(A
   }
 }
 
-// pixels of a sample are shared out so that there are workgroups enough (four a CU; eight are no faster and leave twice the partial sums
-// to join), but never fewer than 32 pixels to one
+// pixels of a sample are shared out so that there are workgroups enough (four a CU; two or three are slower, 4 x 512 x 128 x 127: 119 and 112 us
+// against 109; eight are no faster and leave twice the partial sums to join), but never fewer than 32 pixels to one
 static int chunks_of(int64_t n, int hw) {
   int64_t want = (1024 + n - 1) / n, most = (hw + 31) / 32;
   return (int)(want < 1 ? 1 : want < most ? want : most);

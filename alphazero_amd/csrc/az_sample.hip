@@ -14,11 +14,17 @@
 //
 //   n <= 1,024: a row is one wave's, in registers; the prefix's end is bisected over the score, counting with ballots
 //   longer:     a row is one workgroup's, which walks it twice where it can (the second time it comes from the caches): the first
-//               walk leaves every thread's largest score; what nine sixteenths of these reach (or k of them, for the top k), some 0.8 scores
-//               a thread do where large scores lie anywhere; the second walk lists those in LDS and bounds the mass in f32.  If the prefix ends within the list, the list is sorted and the rest is done on
-//               it.  A longer prefix is found from a histogram linear in the score and a list of the bin it ends in.
+//               walk leaves the largest scores of 1,024 shares of the row; what nine sixteenths of these reach (or k of them, for the top k),
+//               some 820 scores do where large ones lie anywhere; the second walk lists those in LDS and bounds the mass in f32.  If
+//               the prefix ends within the list, the rest is done on it.  A longer prefix is found from a histogram linear in the
+//               score and a list of the bin it ends in.
 //
-// Bound by instructions: about ten a score and walk, and 25 f64 operations an exponential where the kept scores are many.
+// Bound by instructions: about ten a score and walk, and 25 f64 operations an exponential where the kept scores are many.  Measured:
+//   16,384 x 225 f32, masks, top k 16, top p 0.9, min p:   37 us (20.6 k vector instructions a SIMD, 34 us at four cycles each; the 18.6 MB
+//                                                          would take 3.7)
+//   1 x 225 f32:                                           5.4 us, the latency of one wave's steps; the call 12 us
+//   512 x 65,537 bf16, top p 0.9, min p:                   93 us (67 MB: 0.72 TB/s)
+//   1 x 131,072 bf16, top k 50, top p 0.95:                38 us on one CU: a row is not shared out, its sums and lists stay in LDS
 #include "az_ops.hip.h"
 
 namespace azsample {
@@ -568,12 +574,21 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n, walks = (n + NT * V - 1) / (NT * V);
   const Row<T, NT> row{(const T *)a.scores + r * a.stride, a.legal ? a.legal + r * a.legal_stride : nullptr, n, tid, walks};
   const Setting st = setting_of(a, r);
-  uint32_t kmax = KEY_NONE;
-  row.walk([&](const uint32_t *k, int, int) {
+  // the largest of every thread's vectors v, v + G, ..: 1,024 numbers, whatever the workgroup
+  constexpr int G = 1024 / NT;
+  uint32_t kmax = KEY_NONE, own_max[G];
 #pragma unroll
-    for (int j = 0; j < V; ++j) kmax = k[j] > kmax ? k[j] : kmax;
+  for (int q = 0; q < G; ++q) own_max[q] = KEY_NONE;
+  row.walk([&](const uint32_t *k, int, int v) {
+    uint32_t most = k[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) most = k[j] > most ? k[j] : most;
+#pragma unroll
+    for (int q = 0; q < G; ++q)
+      if ((v & (G - 1)) == q) own_max[q] = max(own_max[q], most);
   });
-  const uint32_t own_max = kmax;
+#pragma unroll
+  for (int q = 0; q < G; ++q) kmax = max(kmax, own_max[q]);
   kmax = wave_max(kmax);
   if (lane == 0) sh.kmax[wave] = kmax;
   __syncthreads();
@@ -590,16 +605,17 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   const double m = inf_row ? 0.0 : (double)score_of(kmax);
   const bool cut_k = st.k > 0 && st.k < n, cut_p = st.p < 1.0;
   if ((cut_k || cut_p) && !(cut_k && st.k > LIST)) {
-    // the largest key that nine sixteenths of the threads' largest reach, or, for the top k, that k of them do (all legal scores, if too few hold any)
+    // the largest key that nine sixteenths of those numbers reach, or, for the top k, that k of them do (all legal scores, if too few hold any)
     uint32_t *tops = (uint32_t *)sh.hist;
-    tops[tid] = own_max;
+#pragma unroll
+    for (int q = 0; q < G; ++q) tops[q * NT + tid] = own_max[q];
     if (tid == 0) sh.count = 0;
     __syncthreads();
     if (wave == 0) {
-      uint32_t top[NT / 64], lo = 0xFFFFFFFFu, hi = kmax + 1;
-      const int want = cut_k && st.k < NT * 9 / 16 ? st.k : NT * 9 / 16;
+      uint32_t top[16], lo = 0xFFFFFFFFu, hi = kmax + 1;
+      const int share = min(walks, G) * (NT * 9 / 16), want = cut_k && st.k < share ? st.k : share;
 #pragma unroll
-      for (int j = 0; j < NT / 64; ++j) {
+      for (int j = 0; j < 16; ++j) {
         top[j] = tops[j * 64 + lane];
         lo = min(lo, top[j]);
       }
@@ -608,7 +624,7 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
         const uint32_t mid = lo == KEY_NONE ? lo + (hi - lo) / 2 : middle(lo, hi, step);
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < NT / 64; ++j) c += __popcll(__ballot(top[j] >= mid));
+        for (int j = 0; j < 16; ++j) c += __popcll(__ballot(top[j] >= mid));
         if (c >= want) lo = mid;
         else hi = mid;
         if (c == want) break;
@@ -769,7 +785,11 @@ template <class T, int NT> __global__ __launch_bounds__(NT) void k_sample_block(
   }
 }
 
-// the kernel that holds a row of n scores
+// The kernel that holds a row of n scores.  Measured (us; bf16, top p 0.9 alone / with top k 40):
+//   a wave for up to 1,024: 8,192 x 1,024 f32 52 / 58, a workgroup of 256 86 / 92; 32 scores a lane at 8,192 x 2,048 115 / 124, the workgroup 104 / 100
+//   1,024 threads or 256, four of which share a CU where two of those do: 64 x 5,000 42 / 23 or 28 / 22, 1 x 20,000 62 / 24 or 75 / 20,
+//   1 x 65,537 119 / 26 or 194 / 42, 512 x 20,000 138 / 47 or 94 / 30, 512 x 65,537 264 / 62 or 254 / 49, 2,048 x 65,537 1,044 / 240 or 774 / 144,
+//   512 x 131,072 422 / 77 or 452 / 71 (245 or 363 at temperature 0.7): 256 where rows are short, or fill the card and are not the longest
 template <class T> static void launch_rows(const Args &a, int rows, hipStream_t s) {
   const dim3 four((rows + 3) / 4), one(rows);
   if (a.n <= 64) hipLaunchKernelGGL((k_sample_wave<T, 1>), four, dim3(256), 0, s, a, rows);
@@ -777,7 +797,7 @@ template <class T> static void launch_rows(const Args &a, int rows, hipStream_t 
   else if (a.n <= 256) hipLaunchKernelGGL((k_sample_wave<T, 4>), four, dim3(256), 0, s, a, rows);
   else if (a.n <= 512) hipLaunchKernelGGL((k_sample_wave<T, 8>), four, dim3(256), 0, s, a, rows);
   else if (a.n <= 1024) hipLaunchKernelGGL((k_sample_wave<T, 16>), four, dim3(256), 0, s, a, rows);
-  else if (a.n <= 8192) hipLaunchKernelGGL((k_sample_block<T, 256>), one, dim3(256), 0, s, a);
+  else if (a.n <= 8192 || (rows >= 512 && a.n <= 98304)) hipLaunchKernelGGL((k_sample_block<T, 256>), one, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_sample_block<T, 1024>), one, dim3(1024), 0, s, a);
 }
 

@@ -264,3 +264,16 @@ def test_rows_beyond_32_bit_offsets():
         v, u = rand(rows, n, torch.bfloat16, 55)
         s[:, :n], on[:, :n] = v, torch.rand(rows, n, device="cuda") < 0.5
         check(s[:, :n], u, 0.9, 0, 0.8, 0.0, on[:, :n])
+
+
+@pytest.mark.parametrize("n", [8193, 65537, 131072])
+def test_many_long_rows_draw_what_each_draws_alone(n):
+    """512 rows and more take smaller workgroups: the same actions and log-probabilities, bit for bit"""
+    from alphazero_amd import ops
+
+    s, u = rand(520, n, torch.bfloat16, 78, 3.0)
+    for kw in (dict(top_k=30, top_p=0.9), dict(top_p=0.8), dict(temperature=0.5, min_p=0.01), dict(top_k=2000)):
+        a, lp = ops.sample_actions(s, u, return_logprobs=True, **kw)
+        b, lq = ops.sample_actions(s[:500], u[:500], return_logprobs=True, **kw)
+        assert torch.equal(a[:500], b) and torch.equal(lp[:500], lq)
+    check(s[518:], u[518:].contiguous(), 1.0, 0, 0.8)
