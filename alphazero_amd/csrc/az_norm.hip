@@ -10,8 +10,8 @@
 // a larger one is shared out over workgroups and read twice.  Measured:
 //   1,024 x 128 x 15 x 15 f32, relu, residual: forward 76.7 us (354 MB: 4.6 TB/s), backward 117.8 us (590 MB: 5.0 TB/s) + 5.5 us for dw, db
 //   16,384 x 64 x 15 x 15 bf16, relu, forward: 162 us (944 MB: 5.8 TB/s)
-//   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.4 + 4.0 + 23.4 us, backward 26.4 + 4.9 + 33.4 + 4.2 us (66.6 MB a tensor: 3.3 TB/s over
-//                                              what the passes move; bound by instructions as much, 10 k a SIMD of 4 cycles in backward's)
+//   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.4 + 4.0 + 23.4 us, backward 26.4 + 4.9 + 33.4 + 4.2 us (66.6 MB a tensor: the four
+//                                              passes move 5.0, 5.7, 5.0 and 6.0 TB/s)
 //   64 x 64 x 9 x 9 f32, relu:                 4.2 us, 4.7 + 3.0 us; the call is bound by the host (112 us with autograd's own 72)
 // Mean and variance come from f64 sums of x and x^2 (the products of two f32 are exact in f64, so one pass is enough even where
 // |mean| is 10^5 standard deviations); the mean is kept as a pair of f32 for the subtraction, everything per element is f32, and

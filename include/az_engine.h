@@ -487,8 +487,8 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
  * Adam: training/nn_trainer.py:36-94):
  *   X = M / (|M|_F + eps), on the shorter side;  `steps` times:  A = X X^T,  X = a X + (b A + c A^2) X;  out = X
  * in / out: HOST arrays of `count` device pointers, row-major dense matrices of `dtype` with rows[i] x cols[i] elements (a side of 0:
- * nothing to do; at most 65,536); out[i] may be in[i], and otherwise overlaps no matrix of the call.  f32 and f16 matrices are computed to f32 accuracy (each factor in two f16
- * halves), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
+ * nothing to do; at most 65,536); out[i] may be in[i], and otherwise overlaps no matrix of the call.  f32 and f16 matrices take each factor as two f16 halves (22 bits: errors
+ * like those of f32 products, within a factor of two), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
  * under which a singular value in [0, 1] could grow beyond 7.5 are refused.
  * workspace_dev: az_orthogonalize_workspace() bytes (-1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
  * time need one each.  A matrix's result depends on the others in the call by its last bits at most: calls of matrices no larger than
