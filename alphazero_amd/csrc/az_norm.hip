@@ -13,9 +13,10 @@
 //   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.4 + 4.0 + 23.4 us, backward 26.4 + 4.9 + 33.4 + 4.2 us (66.6 MB a tensor: the four
 //                                              passes move 5.0, 5.7, 5.0 and 6.0 TB/s)
 //   64 x 64 x 9 x 9 f32, relu:                 4.2 us, 4.7 + 3.0 us; the call is bound by the host (112 us with autograd's own 72)
-// Mean and variance come from f64 sums of x and x^2 (the products of two f32 are exact in f64, so one pass is enough even where
-// |mean| is 10^5 standard deviations); the mean is kept as a pair of f32 for the subtraction, everything per element is f32, and
-// each output is rounded once.  A relu's gradient hangs on the sign of z: where f32 cannot tell it, z is recomputed in f64.
+// Mean and variance come from f64 sums of x - p and (x - p)^2 in one pass, p the group's first value (of the sample's first pixel).  p is one
+// of the m values, so (mean - p)^2 <= m var: the sums lose at most a factor of m of f64's 53 bits wherever the values lie (sums of x and x^2
+// lose (mean / deviation)^2 of them), and a flat group has no variance at all.  The mean is kept as a pair of f32 for the subtraction,
+// everything per element is f32, and each output is rounded once.  A relu's gradient hangs on the sign of z: where f32 cannot tell it, z is recomputed in f64.
 // All sums are taken in a fixed order: no atomics.
 #include "az_ops.hip.h"
 
@@ -51,6 +52,8 @@ template <class T, int V> __device__ __forceinline__ void store(T *p, const floa
   for (int j = 0; j < V; ++j) from_f32(o[j], t.v[j]);
   *(Vec<T, V> *)p = t;
 }
+// what a group's sums are taken about: its first value in sample x
+template <class T> __device__ __forceinline__ double pivot_of(const T *x, int g, int cg) { return to_f32(x[g * cg]); }
 template <class T> __device__ __forceinline__ float param(const void *p, int f32, int i, float none) {
   return p == nullptr ? none : f32 ? ((const float *)p)[i] : to_f32(((const T *)p)[i]);
 }
@@ -158,14 +161,16 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_stats(Args 
   for (int c0 = 0; c0 < k.cv; c0 += k.tx_n) {
     const int col = c0 + k.tx;
     double s = 0.0, q = 0.0;
-    if (col < k.cv && k.ty < k.ty_n)
+    if (col < k.cv && k.ty < k.ty_n) {
+      const double pivot = pivot_of(x, col * V / a.cg, a.cg);
 #pragma unroll 4
       for (int p = p0 + k.ty; p < p1; p += k.ty_n) {
         float v[V];
         load<T, V>(v, x + (int64_t)p * a.c + col * V);
 #pragma unroll
-        for (int j = 0; j < V; ++j) { const double d = v[j]; s += d; q = fma(d, d, q); }
+        for (int j = 0; j < V; ++j) { const double d = v[j] - pivot; s += d; q = fma(d, d, q); }
       }
+    }
     s_[tid] = s;
     q_[tid] = q;
     __syncthreads();
@@ -183,15 +188,16 @@ template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_stats(Args 
   }
 }
 
-// mean and 1 / sqrt(var + eps) of m values with sum s and sum of squares q
-__device__ __forceinline__ void finish(double s, double q, double m, double eps, double &mean, double &rstd) {
-  mean = s / m;
+// mean and 1 / sqrt(var + eps) of m values whose differences from the pivot have the sum s and the sum of squares q
+__device__ __forceinline__ void finish(double s, double q, double m, double pivot, double eps, double &mean, double &rstd) {
+  const double off = s / m;
+  mean = pivot + off;
   // a group that holds an infinity or a NaN has no variance (fmax would hide it)
-  rstd = q < 1e300 ? 1.0 / sqrt(fmax(q / m - mean * mean, 0.0) + eps) : NAN;
+  rstd = q < 1e300 ? 1.0 / sqrt(fmax(q / m - off * off, 0.0) + eps) : NAN;
 }
 
 // the chunks' sums -> the statistics: one wave a (sample, group)
-__global__ __launch_bounds__(NT) void k_gn_stats_join(Args a) {
+template <class T> __global__ __launch_bounds__(NT) void k_gn_stats_join(Args a) {
   const int64_t ng = blockIdx.x * (int64_t)(NT / 64) + (threadIdx.x >> 6), n = ng / a.g;
   const int g = (int)(ng - n * a.g), lane = threadIdx.x & 63;
   if (n >= a.n) return;
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(NT) void k_gn_stats_join(Args a) {
   for (int i = lane; i < a.chunks; i += 64) { const double *p = a.part + ((n * a.chunks + i) * a.g + g) * 2; s += p[0]; q += p[1]; }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) { s += __shfl_xor(s, o); q += __shfl_xor(q, o); }
-  if (lane == 0) finish(s, q, (double)a.hw * a.cg, a.eps, a.stats[ng * 2], a.stats[ng * 2 + 1]);
+  if (lane == 0) finish(s, q, (double)a.hw * a.cg, pivot_of((const T *)a.x + n * a.hw * a.c, g, a.cg), a.eps, a.stats[ng * 2], a.stats[ng * 2 + 1]);
 }
 
 template <class T, int V> __global__ __launch_bounds__(NT) void k_gn_apply(Args a) {
@@ -370,7 +376,7 @@ template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_
   const int64_t n = blockIdx.x / a.slices;
   const int col = (int)(blockIdx.x - n * a.slices) * cols + (tid & (cols - 1)), cv = a.c / V, p0 = tid / cols, step = NT / cols;
   // the sample's bytes: a uniform base and a 32-bit offset (a resident sample has at most 1,024 pixels of 64 KiB).  Pixels behind the
-  // sample read its last one; their words are cleared before they count
+  // sample read its last one, and do not count
   const int64_t base = n * a.hw * a.c * (int64_t)sizeof(T);
   const char *x = (const char *)a.x + base, *r = (const char *)a.r + base;
   auto at = [&](int i) { return (uint32_t)(min(p0 + i * step, a.hw - 1) * cv + col) * 16u; };
@@ -381,14 +387,17 @@ template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_
 #pragma unroll
     for (int i = 0; i < NV; ++i) rv[i] = *(const u32x4 *)(r + at(i));
   }
+  const int g = col / cgv;
+  const double pivot = pivot_of((const T *)x, g, a.cg);
   double s = 0.0, q = 0.0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (p0 + i * step >= a.hw) v[i] = u32x4{};
-    float f[V];
-    unpack<T>(v[i], f);
+    if (p0 + i * step < a.hw) {
+      float f[V];
+      unpack<T>(v[i], f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) { const double d = f[j]; s += d; q = fma(d, d, q); }
+      for (int j = 0; j < V; ++j) { const double d = f[j] - pivot; s += d; q = fma(d, d, q); }
+    }
     packed_only(v[i]);
   }
   for (int o = 1; o < 64; o <<= 1)
@@ -402,8 +411,7 @@ template <class T, int NV, bool RES> __global__ __launch_bounds__(NT) void k_gn_
   s = ((part[0][gl][0] + part[1][gl][0]) + part[2][gl][0]) + part[3][gl][0];
   q = ((part[0][gl][1] + part[1][gl][1]) + part[2][gl][1]) + part[3][gl][1];
   double mean, rstd;
-  finish(s, q, (double)a.hw * a.cg, a.eps, mean, rstd);
-  const int g = col / cgv;
+  finish(s, q, (double)a.hw * a.cg, pivot, a.eps, mean, rstd);
   if (tid < cols && (tid & (cgv - 1)) == 0) { a.stats[(n * a.g + g) * 2] = mean; a.stats[(n * a.g + g) * 2 + 1] = rstd; }
   const Stat st = stat_of(mean, rstd);
   char *y = (char *)a.y + base;
@@ -684,7 +692,7 @@ int az_group_norm_forward(int32_t dtype, int32_t param_dtype, int64_t n, int64_t
     constexpr int V = decltype(v)::value;
     const dim3 grid((unsigned)(n * a.chunks));
     hipLaunchKernelGGL((k_gn_stats<T, V>), grid, dim3(NT), 0, s, a);
-    hipLaunchKernelGGL(k_gn_stats_join, dim3((unsigned)((n * groups + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL(k_gn_stats_join<T>, dim3((unsigned)((n * groups + NT / 64 - 1) / (NT / 64))), dim3(NT), 0, s, a);
     hipLaunchKernelGGL((k_gn_apply<T, V>), grid, dim3(NT), 0, s, a);
     return launched("k_gn_forward");
   });
