@@ -1,4 +1,5 @@
-"""ops.group_norm_act's sums where they cancel: flat groups and groups far from zero, against the formulas in float64."""
+"""ops.group_norm_act's sums where they cancel or grow long: flat groups, groups far from zero, and channel sums of many terms of one sign,
+against the formulas in float64."""
 import pytest
 import torch
 
@@ -80,3 +81,23 @@ def test_a_first_value_unlike_the_others():
         y = ops.group_norm_act(x, g, wt, b, activation="none")
         ry = _refs(x, g, wt, b, dy, 1e-5)[0]
         assert bool(((y.double() - ry).abs() <= 2.0 ** -20 * ry.abs() + 2.0 ** -15).all())
+
+
+def test_channel_sums_of_many_terms_of_one_sign():
+    """4,096 pixels of a sample one after the other (129 channels: each thread has one), every term of a channel's sums alike, so that
+    roundings do not cancel.  The f32 runs hold 64 terms at most (64 * 2^-24 of their sum), everything after them is f64 but for three
+    roundings to f32, and xhat carries four: 2^-18 + 7 * 2^-24 < 2^-17"""
+    from alphazero_amd import ops
+
+    n, c, h, w = 1024, 129, 64, 64
+    off = torch.linspace(0.7, 1.3, c, device="cuda") * torch.where(torch.arange(c, device="cuda") % 2 == 0, 1.0, -1.0)
+    x = off.expand(n, h, w, c).contiguous().permute(0, 3, 1, 2)
+    dy = torch.full((n, h, w, c), 1 / 3, device="cuda").permute(0, 3, 1, 2)
+    wt, b = torch.ones(c, device="cuda", requires_grad=True), torch.zeros(c, device="cuda", requires_grad=True)
+    y = ops.group_norm_act(x, 1, wt, b, activation="none")
+    dw, db = torch.autograd.grad(y, [wt, b], dy)
+    each = float(dy[0, 0, 0, 0]) * n * h * w
+    assert float((db.double() - each).abs().max()) <= 2.0 ** -17 * each, float((db.double() / each - 1).abs().max())
+    v = off.double()
+    want = each * (v - v.mean()) / torch.sqrt(((v - v.mean()) ** 2).mean() + 1e-5)
+    assert bool(((dw.double() - want).abs() <= 2.0 ** -17 * want.abs()).all()), float((dw.double() / want - 1).abs().max())
