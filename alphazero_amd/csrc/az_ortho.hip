@@ -103,12 +103,21 @@ template <int P> __device__ __forceinline__ void get8(const _Float16 *o, float *
   for (int e = 0; e < 8; ++e) v[e] = (float)hi[e] + (float)lo[e];
 }
 
+// the workgroups that sum one matrix's squares, 16 Ki elements each: by the matrix alone (the order of a sum is part of its result)
+__host__ __device__ __forceinline__ int parts_of(int rows, int cols) {
+  const int64_t want = ((int64_t)rows * cols + 16383) / 16384;
+  return (int)(want < NORM_PARTS ? want : NORM_PARTS);
+}
+
+// a row of workgroups a matrix, as long as the largest one's
 template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char *ws) {
   __shared__ double s_[NT / 64];
   const int tid = threadIdx.x;
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int i = tid; i < (int)(sizeof(Table) / 4); i += NT) ((uint32_t *)ws)[i] = ((const uint32_t *)&t)[i];
   const Mat m = t.m[blockIdx.y];
+  const int parts = parts_of(m.rows, m.cols);
+  if ((int)blockIdx.x >= parts) return;
   const int64_t n = (int64_t)m.rows * m.cols;
   constexpr int V = 16 / sizeof(T);
   double s = 0.0;
@@ -116,14 +125,14 @@ template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char
   if (((uintptr_t)in & 15) == 0) {
     const int64_t nv = n / V;
 #pragma unroll 4
-    for (int64_t i = blockIdx.x * (int64_t)NT + tid; i < nv; i += (int64_t)gridDim.x * NT) {
+    for (int64_t i = blockIdx.x * (int64_t)NT + tid; i < nv; i += (int64_t)parts * NT) {
       const u32x4 w = ((const u32x4 *)in)[i];
 #pragma unroll
       for (int j = 0; j < V; ++j) { const double v = Word<T>::get(w[j / Word<T>::N], j % Word<T>::N); s = fma(v, v, s); }
     }
     in += nv * V;
   }
-  for (int64_t i = (in - (const T *)m.in) + blockIdx.x * (int64_t)NT + tid; i < n; i += (int64_t)gridDim.x * NT) {
+  for (int64_t i = (in - (const T *)m.in) + blockIdx.x * (int64_t)NT + tid; i < n; i += (int64_t)parts * NT) {
     const double v = to_f32(((const T *)m.in)[i]);
     s = fma(v, v, s);
   }
@@ -154,7 +163,7 @@ __device__ __forceinline__ int find(const Args &a, int kind, int &tile) {
 }
 
 // X0 and its transpose, scaled, split and zero padded: one 64 x 64 tile of X a workgroup
-template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_pack(Args a, int parts) {
+template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_pack(Args a) {
   __shared__ float t_[64][65];
   __shared__ double s_[NT / 64];
   int tile = item_of(a.n[2], blockIdx.x);
@@ -163,7 +172,7 @@ template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_p
   const Mat m = ((const Table *)a.ws)->m[mi];
   const Lay y(m.rows, m.cols, P, PADT);
   char *ws = a.ws + m.ws;
-  double sum = tid < parts ? ((const double *)ws)[tid] : 0.0;
+  double sum = tid < parts_of(m.rows, m.cols) ? ((const double *)ws)[tid] : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if ((tid & 63) == 0) s_[tid >> 6] = sum;
@@ -776,20 +785,17 @@ template <class E, int P> static int run_small(const Args &a, int steps, int cou
 }
 
 template <class E, int P, int T> static int run(const Run &r, Args a, int steps, hipStream_t s) {
-  int64_t most = 0;
+  int parts = 1;
   for (int i = 0; i < r.t.count; ++i) {
-    const int64_t e = (int64_t)r.t.m[i].rows * r.t.m[i].cols;
-    most = e > most ? e : most;
+    const int own = parts_of(r.t.m[i].rows, r.t.m[i].cols);
+    parts = own > parts ? own : parts;
   }
-  // the norm's workgroups: 16 Ki elements each for the largest matrix
-  const int64_t want = (most + 16383) / 16384;
-  const int parts = (int)(want < 1 ? 1 : want < NORM_PARTS ? want : NORM_PARTS);
   a.count = r.t.count;
   a.part = r.part;
   for (int k = 0; k < 6; ++k) a.n[k] = (int)r.n[k];
   const dim3 sym(grid_of(r.n[0])), all(grid_of(r.n[1])), split(grid_of(r.n[5]) + grid_of(r.n[3])), join(grid_of(r.n[4]));
   hipLaunchKernelGGL((k_os_norm<E>), dim3(parts, r.t.count), dim3(NT), 0, s, r.t, a.ws);
-  hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(grid_of(r.n[2])), dim3(NT), 0, s, a, parts);
+  hipLaunchKernelGGL((k_os_pack<E, P, T>), dim3(grid_of(r.n[2])), dim3(NT), 0, s, a);
   for (int k = 0; k < steps; ++k) {
     a.cur = k & 1;
     if (r.n[3]) {

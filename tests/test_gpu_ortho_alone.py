@@ -1,0 +1,32 @@
+"""ops.orthogonalize: what a matrix's result may and may not owe to the others of its call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from .test_gpu_ortho import COEF, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _norm_sums(ms):
+    """the first matrix's 256 partial sums of squares, as a call of the C entry leaves them: the workspace begins with a table of
+    (in, out, byte offset of the buffers, rows, cols), and a matrix's buffers with these sums"""
+    from alphazero_amd.engine import load_library
+
+    lib, n = load_library(), len(ms)
+    rows, cols = (C.c_int32 * n)(*[m.shape[0] for m in ms]), (C.c_int32 * n)(*[m.shape[1] for m in ms])
+    out = [torch.empty_like(m) for m in ms]
+    ws = torch.zeros(lib.az_orthogonalize_workspace(0, n, rows, cols), dtype=torch.uint8, device="cuda")
+    ptrs = lambda ts: (C.c_void_p * n)(*[t.data_ptr() for t in ts])
+    assert lib.az_orthogonalize(0, n, ptrs(ms), ptrs(out), rows, cols, 1, *COEF, 1e-7, ws.data_ptr(), ws.numel(),
+                                torch.cuda.current_stream().cuda_stream) == 0
+    at = int(ws[16:24].view(torch.int64))
+    return ws[at:at + 2048].view(torch.float64).clone()
+
+
+def test_a_norm_is_summed_in_the_same_order_beside_larger_matrices():
+    m, larger = make((100, 200), torch.float32, 1), make((700, 3000), torch.float32, 2)
+    alone = _norm_sums([m])
+    assert abs(float(alone.sum()) / float((m.double() ** 2).sum()) - 1) < 1e-12
+    assert torch.equal(alone, _norm_sums([m, larger]))
