@@ -120,20 +120,18 @@ template <class T> __global__ __launch_bounds__(NT) void k_os_norm(Table t, char
   if ((int)blockIdx.x >= parts) return;
   const int64_t n = (int64_t)m.rows * m.cols;
   constexpr int V = 16 / sizeof(T);
+  const int64_t nv = n / V;
   double s = 0.0;
   const T *in = (const T *)m.in;
-  if (((uintptr_t)in & 15) == 0) {
-    const int64_t nv = n / V;
 #pragma unroll 4
-    for (int64_t i = blockIdx.x * (int64_t)NT + tid; i < nv; i += (int64_t)parts * NT) {
-      const u32x4 w = ((const u32x4 *)in)[i];
+  for (int64_t i = blockIdx.x * (int64_t)NT + tid; i < nv; i += (int64_t)parts * NT) {
+    u32x4 w;
+    __builtin_memcpy(&w, in + i * V, 16);  // (aligned to its elements only)
 #pragma unroll
-      for (int j = 0; j < V; ++j) { const double v = Word<T>::get(w[j / Word<T>::N], j % Word<T>::N); s = fma(v, v, s); }
-    }
-    in += nv * V;
+    for (int j = 0; j < V; ++j) { const double v = Word<T>::get(w[j / Word<T>::N], j % Word<T>::N); s = fma(v, v, s); }
   }
-  for (int64_t i = (in - (const T *)m.in) + blockIdx.x * (int64_t)NT + tid; i < n; i += (int64_t)parts * NT) {
-    const double v = to_f32(((const T *)m.in)[i]);
+  for (int64_t i = nv * V + blockIdx.x * (int64_t)NT + tid; i < n; i += (int64_t)parts * NT) {
+    const double v = to_f32(in[i]);
     s = fma(v, v, s);
   }
 #pragma unroll

@@ -30,3 +30,12 @@ def test_a_norm_is_summed_in_the_same_order_beside_larger_matrices():
     alone = _norm_sums([m])
     assert abs(float(alone.sum()) / float((m.double() ** 2).sum()) - 1) < 1e-12
     assert torch.equal(alone, _norm_sums([m, larger]))
+
+
+def test_a_norm_is_summed_in_the_same_order_at_any_address():
+    m = make((100, 203), torch.float32, 3)
+    store = torch.empty(m.numel() + 3, device="cuda")
+    for off in (1, 2, 3):
+        moved = store[off:off + m.numel()].view(m.shape)
+        moved.copy_(m)
+        assert torch.equal(_norm_sums([moved]), _norm_sums([m]))
