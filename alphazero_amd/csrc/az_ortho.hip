@@ -7,12 +7,12 @@
 // from the symmetric A with itself, B X from B and the transpose of X, which every step writes beside X.  Of the symmetric results
 // only the tiles that touch the upper triangle are computed; the lower one is its mirror image.
 //
-// Arithmetic: f16 matrix instructions with f32 sums.  For f32 and f16 matrices an operand is a pair of f16, hi = f16(v) and
-// lo = f16(v - hi), and a product is hi hi + hi lo + lo hi: 22 bits of each factor, three matrix instructions, several times the rate
-// of the f32 ones.  For bf16 matrices hi alone holds more (11 bits) than the result will (8).  Stored values are scaled by powers of
-// two, as large as the host's bound on the singular values allows (az_orthogonalize: entries stay below 2^15), which keeps lo clear
-// of f16's smallest steps.  Buffers are zero padded to whole tiles and the padding stays
-// zero: no product has a border case.
+// Arithmetic: f16 matrix instructions with f32 sums.  An operand is a pair of f16, hi = f16(v) and lo = f16(v - hi), and a product is
+// hi hi + hi lo + lo hi: 22 bits of each factor, three matrix instructions, several times the rate of the f32 ones.  For bf16 matrices
+// with a short side beyond 64 hi alone holds more (11 bits) than the result will (8; what that costs stands at planes_of).  Stored values
+// are scaled by powers of two, as large as the host's bound on the singular values allows (az_orthogonalize: entries stay below 2^15),
+// which keeps lo clear of f16's smallest steps.  Buffers are zero padded to whole tiles and the padding stays zero: no product has a
+// border case.
 //
 // A row of an operand is a run of 128-byte units: 64 k of hi, or hi and lo of 32 k.  A stage of a product is one unit of every row of
 // the two panels, moved straight from memory to LDS (16 bytes a lane) while the stage before it is multiplied.  Unit r's 16-byte
@@ -440,19 +440,19 @@ struct SmallTable {
 // piece q (four halves) of row r of a 64 x 64 f16 plane; the pieces of 16 rows fall on different banks
 __device__ __forceinline__ int piece(int r, int q) { return r * 64 + ((q ^ (r & 15)) << 2); }
 
-template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_os_small(SmallTable t, float ca, float cb, float cc, double eps, float sx, float sa, float sb, int steps) {
+template <class E, int RB> __global__ __launch_bounds__(SMALL_NT) void k_os_small(SmallTable t, float ca, float cb, float cc, double eps, float sx, float sa, float sb, int steps) {
   constexpr int TILES = RB == 1 ? 1 : 3;
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILES * 16 * 64 * 4 + 64 * 64 * 2 * P];
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILES * 16 * 64 * 4 + 64 * 64 * 4];
   float *part = (float *)lds;                                         // [slot 4][tile][element 16][lane]
   _Float16 *am = (_Float16 *)(lds + 4 * TILES * 16 * 64 * 4);         // A: planes of 64 x 64
   _Float16 *bm = (_Float16 *)lds;                                     // B: over the partial sums, which have been read by then
-  static_assert(64 * 64 * 2 * P <= 4 * TILES * 16 * 64 * 4, "B fits the partial sums' memory");
+  static_assert(64 * 64 * 4 <= 4 * TILES * 16 * 64 * 4, "B fits the partial sums' memory");
   const Mat m = t.m[blockIdx.x];
   const bool tall = m.rows > m.cols;
   const int S = tall ? m.cols : m.rows, L = tall ? m.rows : m.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hf = lane >> 5, l32 = lane & 31;
   const int blocks = (L + 31) / 32, nb = wave < blocks ? (blocks - wave + 7) / 8 : 0;
-  u32x4 x[SMALL_NB][RB][2][P];  // [block][32 rows][chunk of 16 rows][hi, lo], two f16 a word
+  u32x4 x[SMALL_NB][RB][2][2];  // [block][32 rows][chunk of 16 rows][hi, lo], two f16 a word
   f32x16 raw[SMALL_NB][RB];
   double sum = 0.0;
 #pragma unroll
@@ -480,16 +480,16 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
   const double norm = sqrt(sum) + eps;
   const double scale = norm < 1e300 ? (norm > 0.0 ? (double)sx / norm : 0.0) : NAN;  // (no finite norm: no result)
   typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
-  auto keep = [&](u32x4 (&o)[2][P], int e, float v0, float v1) {  // elements e and e + 1
+  auto keep = [&](u32x4 (&o)[2][2], int e, float v0, float v1) {  // elements e and e + 1
     const half2_ hi = {(_Float16)v0, (_Float16)v1};
     o[e >> 3][0][(e & 7) >> 1] = __builtin_bit_cast(uint32_t, hi);
-    if (P == 2) o[e >> 3][P - 1][(e & 7) >> 1] = __builtin_bit_cast(uint32_t, half2_{(_Float16)(v0 - (float)hi[0]), (_Float16)(v1 - (float)hi[1])});
+    o[e >> 3][1][(e & 7) >> 1] = __builtin_bit_cast(uint32_t, half2_{(_Float16)(v0 - (float)hi[0]), (_Float16)(v1 - (float)hi[1])});
   };
-  auto packed = [&](u32x4 (&o)[2][P]) {  // (whole words from here on, not an element a register)
+  auto packed = [&](u32x4 (&o)[2][2]) {  // (whole words from here on, not an element a register)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int h = 0; h < P; ++h) asm volatile("" : "+v"(o[c][h]));
+      for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(o[c][h]));
   };
 #pragma unroll
   for (int b = 0; b < SMALL_NB; ++b)
@@ -527,12 +527,12 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
       }
       const int j = tj * 32 + l32, i = ti * 32 + e4 * 8 + hf * 4;
       *(half4 *)(p + piece(j, i >> 2)) = hi;
-      if (P == 2) *(half4 *)(p + 4096 + piece(j, i >> 2)) = lo;
+      *(half4 *)(p + 4096 + piece(j, i >> 2)) = lo;
       if (ti != tj) {
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           p[piece(i + d, j >> 2) + (j & 3)] = hi[d];
-          if (P == 2) p[4096 + piece(i + d, j >> 2) + (j & 3)] = lo[d];
+          p[4096 + piece(i + d, j >> 2) + (j & 3)] = lo[d];
         }
       }
     }
@@ -543,11 +543,11 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
 #pragma unroll
     for (int b = 0; b < SMALL_NB; ++b) {
       if (b >= nb) continue;
-      half8 xt[RB][2][P];
+      half8 xt[RB][2][2];
 #pragma unroll
       for (int r = 0; r < RB; ++r)
 #pragma unroll
-        for (int h = 0; h < P; ++h) {
+        for (int h = 0; h < 2; ++h) {
           f32x16 d = {};
           d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x[b][r][0][h]), one[0], d, 0, 0, 0);
           d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x[b][r][1][h]), one[1], d, 0, 0, 0);
@@ -565,10 +565,8 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
         const int ti = q == 2 ? 1 : 0, tj = q == 0 ? 0 : 1;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (P == 2) {
-            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][P - 1], xt[RB == 1 ? 0 : tj][c][0], acc[q], 0, 0, 0);
-            acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][0], xt[RB == 1 ? 0 : tj][c][P - 1], acc[q], 0, 0, 0);
-          }
+          acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][1], xt[RB == 1 ? 0 : tj][c][0], acc[q], 0, 0, 0);
+          acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][0], xt[RB == 1 ? 0 : tj][c][1], acc[q], 0, 0, 0);
           acc[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xt[ti][c][0], xt[RB == 1 ? 0 : tj][c][0], acc[q], 0, 0, 0);
         }
       }
@@ -606,13 +604,11 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
       f32x16 d = {};
 #pragma unroll
       for (int c = 0; c < 2 * RB; ++c) {
-        half8 p[P], q[P];
+        half8 p[2], q[2];
 #pragma unroll
-        for (int h = 0; h < P; ++h) { p[h] = rows_of(am, ti, c, h); q[h] = rows_of(am, tj, c, h); }
-        if (P == 2) {
-          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], q[0], d, 0, 0, 0);
-          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], q[P - 1], d, 0, 0, 0);
-        }
+        for (int h = 0; h < 2; ++h) { p[h] = rows_of(am, ti, c, h); q[h] = rows_of(am, tj, c, h); }
+        d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[1], q[0], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], q[1], d, 0, 0, 0);
         d = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], q[0], d, 0, 0, 0);
       }
       const float f = cc * (sb / (sa * sa)), g = cb * (sb / sa);
@@ -632,13 +628,11 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
       for (int r = 0; r < RB; ++r)
 #pragma unroll
         for (int c = 0; c < 2 * RB; ++c) {
-          half8 p[P];
+          half8 p[2];
 #pragma unroll
-          for (int h = 0; h < P; ++h) p[h] = rows_of(bm, r, c, h);
-          if (P == 2) {
-            d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[P - 1], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][0]), d[r], 0, 0, 0);
-            d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][P - 1]), d[r], 0, 0, 0);
-          }
+          for (int h = 0; h < 2; ++h) p[h] = rows_of(bm, r, c, h);
+          d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[1], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][0]), d[r], 0, 0, 0);
+          d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][1]), d[r], 0, 0, 0);
           d[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0], __builtin_bit_cast(half8, x[b][c >> 1][c & 1][0]), d[r], 0, 0, 0);
         }
 #pragma unroll
@@ -650,7 +644,7 @@ template <class E, int P, int RB> __global__ __launch_bounds__(SMALL_NT) void k_
             const uint32_t word = x[b][r][e >> 3][h][(e & 7) >> 1];  // (a bit cast of the vector's element itself reads element 0)
             return (float)__builtin_bit_cast(half2_, word)[e & 1];
           };
-          v[e] = fmaf(ca, P == 2 ? half_at(0) + half_at(P - 1) : half_at(0), d[r][e] * inv);
+          v[e] = fmaf(ca, half_at(0) + half_at(1), d[r][e] * inv);
         }
         if (!last) {
 #pragma unroll
@@ -676,17 +670,27 @@ static bool is_small(int rows, int cols) {
   return s <= SMALL_S && l <= SMALL_L;
 }
 
+// f16 halves a factor is held in.  bf16 matrices with a short side beyond 64 make do with one: the errors of 11-bit factors, beside the 8-bit result's own
+// rounding of 1.66e-3 (relative, Frobenius), come to 2.0e-3 .. 2.8e-3 in all (4096 x 4096 1.98e-3; short sides of 80 to 200 the most).  On short sides
+// of 64 and less there are too few directions for them to average out (64 x 576 4.1e-3, 1 x 7 6.3e-3), and a second half costs little (64 x 576 alone
+// 34 -> 55 us; 1536 x 1536 would take 470 instead of 250).
+static int planes_of(int32_t dtype, int rows, int cols) { return dtype == AZ_NN_BF16 && (rows < cols ? rows : cols) > SMALL_S ? 1 : 2; }
+
 static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }
 
 // tile side by the short side: measured on 1536 x 1536 / 2000 x 4096, 64 takes 0.47 / 1.54 ms in f32 and 0.25 / 0.76 ms in bf16, 128 takes
 // 0.53 / 1.34 and 0.34 / 0.59
 static int tile_of(int rows, int cols) { return (rows < cols ? rows : cols) >= 1792 ? 128 : 64; }
 
-// One workgroup a matrix where every matrix of the call is small; beside larger ones they cost nothing in the others' launches, and a
-// launch of their own would (64 x 576 f32 alone: 88 us in 17 launches, 54 in one).
-static bool all_small(int count, const int32_t *rows, const int32_t *cols) {
+static bool in_class(int32_t dtype, int rows, int cols, int planes, int tile) {
+  return rows > 0 && cols > 0 && planes_of(dtype, rows, cols) == planes && tile_of(rows, cols) == tile;
+}
+
+// One workgroup a matrix where every matrix that would share the launches of the others (two halves, tiles of 64) is small; beside larger ones
+// they cost nothing in those launches, and a launch of their own would (64 x 576 f32 alone: 88 us in 17 launches, 54 in one).
+static bool all_small(int32_t dtype, int count, const int32_t *rows, const int32_t *cols) {
   for (int i = 0; i < count; ++i)
-    if (rows[i] > 0 && cols[i] > 0 && !is_small(rows[i], cols[i])) return false;
+    if (in_class(dtype, rows[i], cols[i], 2, 64) && !is_small(rows[i], cols[i])) return false;
   return true;
 }
 
@@ -722,25 +726,28 @@ static bool bounded(int steps, double a, double b, double c, Args &g) {
   return true;
 }
 
-// One run of launches: up to MAX_M matrices of one tile size, and where everything lies in the workspace.
+// One run of launches: up to MAX_M matrices of one tile size and number of halves, and where everything lies in the workspace.
 struct Run {
   Table t;
-  int tile;
+  int planes, tile;
   uint32_t n[6];
   uint64_t part, bytes;
 };
 
-// f(Run &) for every run of the call; in / out may be null (sizes only)
-template <class F> static int each_run(int planes, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, F f) {
-  for (int tile = 64; tile <= 128; tile *= 2) {
+// f(Run &) for every run of the call but the small matrices' where k_os_small takes those; in / out may be null (sizes only)
+template <class F> static int each_run(int32_t dtype, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, F f) {
+  const bool small = all_small(dtype, count, rows, cols);
+  for (int kind = small ? 1 : 0; kind < 4; ++kind) {
+    const int planes = kind < 2 ? 2 : 1, tile = kind & 1 ? 128 : 64;
     Run r;
     r.t.count = 0;
     for (int i = 0; i < count; ++i) {
-      if (rows[i] > 0 && cols[i] > 0 && tile_of(rows[i], cols[i]) == tile) {
+      if (in_class(dtype, rows[i], cols[i], planes, tile)) {
         r.t.m[r.t.count++] = Mat{in ? in[i] : nullptr, out ? out[i] : nullptr, 0, rows[i], cols[i]};
       }
       if (r.t.count == 0 || (r.t.count < MAX_M && i < count - 1)) continue;
       uint64_t off = round_up(sizeof(Table));
+      r.planes = planes;
       r.tile = tile;
       for (uint32_t &v : r.n) v = 0;
       for (int k = 0; k < r.t.count; ++k) {
@@ -766,16 +773,16 @@ template <class F> static int each_run(int planes, int count, const void *const 
   return AZ_OK;
 }
 
-template <class E, int P> static int run_small(const Args &a, int steps, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, hipStream_t s) {
+template <class E> static int run_small(const Args &a, int steps, int count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols, hipStream_t s) {
   for (int rb = 1; rb <= 2; ++rb) {
     SmallTable t;
     int n = 0;
     for (int i = 0; i < count; ++i) {
       const int side = rows[i] < cols[i] ? rows[i] : cols[i];
-      if (side > 0 && (side <= 32) == (rb == 1)) t.m[n++] = Mat{in[i], out[i], 0, rows[i], cols[i]};
+      if (side > 0 && is_small(rows[i], cols[i]) && (side <= 32) == (rb == 1)) t.m[n++] = Mat{in[i], out[i], 0, rows[i], cols[i]};
       if (n == 0 || (n < MAX_M && i < count - 1)) continue;
-      if (rb == 1) hipLaunchKernelGGL((k_os_small<E, P, 1>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
-      else hipLaunchKernelGGL((k_os_small<E, P, 2>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
+      if (rb == 1) hipLaunchKernelGGL((k_os_small<E, 1>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
+      else hipLaunchKernelGGL((k_os_small<E, 2>), dim3(n), dim3(SMALL_NT), 0, s, t, a.a, a.b, a.c, a.eps, a.sx, a.sa, a.sb, steps);
       n = 0;
     }
   }
@@ -824,9 +831,8 @@ int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *
   using namespace azortho;
   const char *msg = "";
   if (check(msg, dtype, count, rows, cols) != AZ_OK) { fail(AZ_EINVAL, msg); return -1; }
-  if (all_small(count, rows, cols)) return 0;
   uint64_t most = 0;  // (runs follow each other on the stream: they share the memory)
-  each_run(dtype == AZ_NN_BF16 ? 1 : 2, count, nullptr, nullptr, rows, cols, [&](const Run &r) {
+  each_run(dtype, count, nullptr, nullptr, rows, cols, [&](const Run &r) {
     most = r.bytes > most ? r.bytes : most;
     return AZ_OK;
   });
@@ -842,7 +848,7 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
   if (!(eps >= 0.0 && eps < 1e300)) return fail(AZ_EINVAL, "orthogonalize: eps >= 0");
   Args g{};
   if (!bounded(steps, a, b, c, g)) return fail(AZ_EINVAL, "orthogonalize: these coefficients let singular values grow beyond 7.5 (or the polynomial beyond 100)");
-  const int es = dtype == AZ_NN_F32 ? 4 : 2, planes = dtype == AZ_NN_BF16 ? 1 : 2;
+  const int es = dtype == AZ_NN_F32 ? 4 : 2;
   if (count > 0 && (!in || !out)) return fail(AZ_EINVAL, "orthogonalize: null argument");
   int live = 0;
   for (int i = 0; i < count; ++i) {
@@ -851,20 +857,23 @@ int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *
     if (!in[i] || !out[i] || misaligned(in[i], es) || misaligned(out[i], es)) return fail(AZ_EINVAL, "orthogonalize: null or misaligned matrix");
   }
   if (live == 0) return AZ_OK;
-  const bool small = all_small(count, rows, cols);
-  if (!small && (!workspace_dev || misaligned(workspace_dev, 256) || workspace_bytes < az_orthogonalize_workspace(dtype, count, rows, cols)))
+  const int64_t need = az_orthogonalize_workspace(dtype, count, rows, cols);
+  if (need > 0 && (!workspace_dev || misaligned(workspace_dev, 256) || workspace_bytes < need))
     return fail(AZ_EINVAL, "orthogonalize: workspace below az_orthogonalize_workspace() or not aligned to 256 bytes");
   hipStream_t s = (hipStream_t)stream;
   DeviceGuard guard(s);
   if (!guard.ok) return fail(AZ_EHIP, "orthogonalize: cannot select the stream's device");
   g.ws = (char *)workspace_dev;
   g.a = (float)a; g.b = (float)b; g.c = (float)c; g.eps = eps;
-  if (small)
-    return dtype == AZ_NN_F32 ? run_small<float, 2>(g, steps, count, in, out, rows, cols, s) : dtype == AZ_NN_BF16 ? run_small<bf16_t, 1>(g, steps, count, in, out, rows, cols, s)
-                                                                                                                  : run_small<f16_t, 2>(g, steps, count, in, out, rows, cols, s);
-  return each_run(planes, count, in, out, rows, cols, [&](const Run &r) {
-    if (r.tile == 64) return dtype == AZ_NN_F32 ? run<float, 2, 64>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 64>(r, g, steps, s) : run<f16_t, 2, 64>(r, g, steps, s);
-    return dtype == AZ_NN_F32 ? run<float, 2, 128>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 1, 128>(r, g, steps, s) : run<f16_t, 2, 128>(r, g, steps, s);
+  if (all_small(dtype, count, rows, cols)) {
+    const int rc = dtype == AZ_NN_F32 ? run_small<float>(g, steps, count, in, out, rows, cols, s) : dtype == AZ_NN_BF16 ? run_small<bf16_t>(g, steps, count, in, out, rows, cols, s)
+                                                                                                                : run_small<f16_t>(g, steps, count, in, out, rows, cols, s);
+    if (rc != AZ_OK) return rc;
+  }
+  return each_run(dtype, count, in, out, rows, cols, [&](const Run &r) {
+    if (r.planes == 1) return r.tile == 64 ? run<bf16_t, 1, 64>(r, g, steps, s) : run<bf16_t, 1, 128>(r, g, steps, s);
+    if (r.tile == 64) return dtype == AZ_NN_F32 ? run<float, 2, 64>(r, g, steps, s) : dtype == AZ_NN_BF16 ? run<bf16_t, 2, 64>(r, g, steps, s) : run<f16_t, 2, 64>(r, g, steps, s);
+    return dtype == AZ_NN_F32 ? run<float, 2, 128>(r, g, steps, s) : run<f16_t, 2, 128>(r, g, steps, s);
   });
 }
 

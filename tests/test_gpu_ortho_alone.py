@@ -1,10 +1,11 @@
-"""ops.orthogonalize: what a matrix's result may and may not owe to the others of its call."""
+"""ops.orthogonalize: what a matrix's result may and may not owe to the others of its call, and how exact bf16 results of short sides are."""
 import ctypes as C
+import math
 
 import pytest
 import torch
 
-from .test_gpu_ortho import COEF, make
+from .test_gpu_ortho import COEF, make, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,22 @@ def test_a_norm_is_summed_in_the_same_order_at_any_address():
         moved = store[off:off + m.numel()].view(m.shape)
         moved.copy_(m)
         assert torch.equal(_norm_sums([moved]), _norm_sums([m]))
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (7, 1), (20, 700), (32, 768), (33, 32), (768, 33), (64, 64), (64, 576), (64, 769), (2, 3000), (4096, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_bf16_results_of_short_sides_are_off_by_their_own_rounding(shape):
+    """Factors of 22 bits leave the result x + d before its rounding; |round(x + d) - x| <= |round(x) - x| + 2 |d| entry by entry.  d: four
+    times the larger of two runs of the definition whose X, A and B carry errors of that size (as in test_gpu_ortho)"""
+    from alphazero_amd import ops
+
+    level = 2.0 ** -22 + 2.0 ** -24 * math.sqrt(max(shape))
+    larger = make((100, 900), torch.bfloat16, 77)
+    for seed in range(4):
+        m = make(shape, torch.bfloat16, seed * 131 + shape[0], 0.01)
+        ref = plain(m)
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        d = 4 * max(float((plain(m, noise=level, gen=gen) - ref).norm()) for _ in range(2))
+        own = float((ref.bfloat16().double() - ref).norm())
+        for got in (ops.orthogonalize(m), ops.orthogonalize([larger, m])[1]):
+            err = float((got.double() - ref).norm())
+            assert err <= own + 2 * d + 2.0 ** -24, (err, own, d)
