@@ -487,12 +487,16 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
  * Adam: training/nn_trainer.py:36-94):
  *   X = M / (|M|_F + eps), on the shorter side;  `steps` times:  A = X X^T,  X = a X + (b A + c A^2) X;  out = X
  * in / out: HOST arrays of `count` device pointers, row-major dense matrices of `dtype` with rows[i] x cols[i] elements (a side of 0:
- * nothing to do; at most 65,536); out[i] may be in[i], and otherwise overlaps no matrix of the call.  f32 and f16 matrices take each factor as two f16 halves (22 bits: errors
- * like those of f32 products, within a factor of two), bf16 ones with f16 factors; sums are f32.  A matrix with an infinity or a NaN gives NaN, a zero matrix zeros.  Coefficients
- * under which a singular value in [0, 1] could grow beyond 7.5 are refused.
- * workspace_dev: az_orthogonalize_workspace() bytes (-1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
- * time need one each.  A matrix's result depends on the others in the call by its last bits at most: calls of matrices no larger than
- * 64 x 768 alone take another kernel (and no workspace). */
+ * nothing to do; at most 65,536); out[i] may be in[i], and otherwise overlaps no matrix of the call.  Sums are f32.  Factors are two f16
+ * halves (22 bits: errors like those of f32 products, within a factor of two), of bf16 matrices with a short side beyond 64 one (11 bits:
+ * 1.2 .. 1.7 times the error of the result's own rounding in all).  Entries of X below 2^-16 keep fewer bits (they stand in steps of 2^-38 with the
+ * usual coefficients): a matrix whose norm is far below eps loses accuracy.  A matrix with an infinity or a NaN gives NaN, a zero matrix
+ * zeros.  Coefficients under which a singular value in [0, 1] could grow beyond 7.5 are refused.
+ * A matrix's result does not depend on the others of the call, but for matrices of at most 64 x 768: beside a larger one (of bf16 matrices:
+ * beside a longer one with a short side of at most 64) they take another kernel, whose sums run in another order.  Either result is as exact as
+ * said above, and they differ by as much (64 x 576 f32: by up to 2e-6 of the result's norm, the error of either).
+ * workspace_dev: az_orthogonalize_workspace() bytes (0: none; -1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
+ * time need one each. */
 int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols);
 int az_orthogonalize(int32_t dtype, int32_t count, const void *const *in, void *const *out, const int32_t *rows, const int32_t *cols,
                      int32_t steps, double a, double b, double c, double eps, void *workspace_dev, int64_t workspace_bytes, void *stream);

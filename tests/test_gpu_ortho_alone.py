@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_ortho import COEF, make, plain
+from .test_gpu_ortho import COEF, SHAPES, check, make, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,46 @@ def test_bf16_results_of_short_sides_are_off_by_their_own_rounding(shape):
         for got in (ops.orthogonalize(m), ops.orthogonalize([larger, m])[1]):
             err = float((got.double() - ref).norm())
             assert err <= own + 2 * d + 2.0 ** -24, (err, own, d)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_small_matrices_beside_larger_ones_against_the_definition(dtype):
+    """in one call with a larger matrix they take another kernel than alone; both are held to the definition"""
+    from alphazero_amd import ops
+
+    small = [make(s, dtype, i, 0.01) for i, s in enumerate(s for s in SHAPES if min(s) <= 64 and max(s) <= 768)]
+    assert len(small) > 12
+    for larger in (make((100, 900), dtype, 78), make((60, 900), dtype, 79)):
+        got = ops.orthogonalize([*small, larger])
+        for m, o, alone in zip(small, got, ops.orthogonalize(small)):
+            check(m, o)
+            check(m, alone)
+        assert torch.equal(got[-1], ops.orthogonalize(larger))
+
+
+@pytest.mark.parametrize("shape", [(64, 100), (100, 200)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("k", [14, 20, 26, 40])
+def test_norms_far_below_eps(shape, k):
+    """|M| = 2^-k eps: X0 is about 2^-k, every step multiplies it by 3.4445 (its cube is far below it).  Entries of X stand in steps of 2^-38
+    (2^-24 over the scale 2^14), so that 2^-39 may be lost at X0 and at each step, and 3.4445^5 (1 + 1 / 3.4445 + ..) = 684 times that in
+    all; beside it five times the 2^-22 of the halves and the 2^-23 of f32 arithmetic"""
+    from alphazero_amd import ops
+
+    eps = 1e-7
+    m = make(shape, torch.float32, 5)
+    m = m * float(eps * 2.0 ** -k / m.double().norm())
+    ref = plain(m, eps=eps)
+    got = ops.orthogonalize(m, eps=eps)
+    assert bool(((got.double() - ref).abs() <= 2.0 ** -19 * ref.abs() + 684 * 2.0 ** -39).all()), float((got.double() - ref).abs().max())
+    assert k == 40 or float(got.abs().max()) > 0
+
+
+def test_buffers_that_start_beyond_4_gib():
+    """a 4,096 x 65,536 f32 matrix has 3.1 GiB of the workspace (X, two transposes, A, B): the third one's begin past 6 GiB, and its result is the
+    same, bit for bit"""
+    from alphazero_amd import ops
+
+    m = torch.randn(4096, 65536, device="cuda", generator=torch.Generator(device="cuda").manual_seed(72))
+    one = ops.orthogonalize(m, steps=1)
+    for o in ops.orthogonalize([m, m, m], steps=1):
+        assert torch.equal(o, one)
