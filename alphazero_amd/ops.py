@@ -19,19 +19,17 @@ def _check(rc: int) -> None:
         raise EngineError(f"az call failed ({rc}): {load_library().az_tower_last_error().decode()}")
 
 
-# (the stream and the device without the Python objects around them: 8 us less a call in autograd's thread)
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
-
+# The stream and the device without the Python objects around them: 8 us less a call in autograd's thread.  (Looked up in the call: a torch
+# without GPU support has neither, and this module is imported there too.)
 def _stream(device: torch.device) -> C.c_void_p:
-    return C.c_void_p(_raw_stream(device.index))
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 class _on:
     """the device current for the allocations inside, without a switch where it is current already"""
 
     def __init__(self, device: torch.device):
-        self.guard = None if _current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
