@@ -12,6 +12,7 @@ SRCS = [os.path.join(_HERE, "csrc", "az_engine.hip"), os.path.join(_HERE, "csrc"
         os.path.join(_HERE, "csrc", "az_norm.hip"), os.path.join(_HERE, "csrc", "az_ortho.hip")]
 DEPS = [*SRCS, os.path.join(_HERE, "csrc", "az_games.hip.h"), os.path.join(_HERE, "csrc", "az_ops.hip.h"),
         os.path.join(os.path.dirname(_HERE), "include", "az_engine.h")]
+RECIPE = os.path.abspath(__file__)  # (FLAGS stand here)
 LIB_DIR = os.path.join(_HERE, "lib")
 # AZ_ENGINE_LIB: load another build of the library instead (A/B measurements of kernel variants: scripts/dev/build_variant.sh)
 LIB = os.environ.get("AZ_ENGINE_LIB") or os.path.join(LIB_DIR, "libaz_engine.so")
@@ -22,14 +23,23 @@ FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-ffp-contract=o
          "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-int-to-void-pointer-cast",
          # no packed f32 arithmetic: some of its forms are not safe on this card (the host pass warns that it does not know the feature)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-OBJ_DIR = os.path.join(LIB_DIR, "obj")  # per-source objects (git-ignored): only what changed is recompiled
+# per-source objects, each with the flags it was compiled with beside it (git-ignored): only what changed is recompiled
+OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
 
 def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(d) > t for d in DEPS if os.path.exists(d))
+    return any(os.path.getmtime(d) > t for d in [*DEPS, RECIPE] if os.path.exists(d))
+
+
+def _flags_of(obj: str) -> str | None:
+    try:
+        with open(obj + ".flags") as f:
+            return f.read()
+    except OSError:
+        return None
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -43,14 +53,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
         obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
         objs.append(obj)
         newest = max(os.path.getmtime(f) for f in [src, *headers] if os.path.exists(f))
-        if force or not os.path.exists(obj) or os.path.getmtime(obj) < newest:
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < newest or _flags_of(obj) != " ".join(FLAGS):
             cmd = [hipcc, *FLAGS, "-c", "-o", obj, src]
             if verbose:
                 print(" ".join(cmd))
-            jobs.append((cmd, subprocess.Popen(cmd)))
-    for cmd, p in jobs:
+            jobs.append((cmd, obj, subprocess.Popen(cmd)))
+    for cmd, obj, p in jobs:
         if p.wait() != 0:
             raise subprocess.CalledProcessError(p.returncode, cmd)
+        with open(obj + ".flags", "w") as f:
+            f.write(" ".join(FLAGS))
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
     if verbose:
         print(" ".join(cmd))
