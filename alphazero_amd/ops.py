@@ -3,7 +3,7 @@ scores (``sample_actions``), the normalisation layer of a residual tower with it
 weight update (``orthogonalize``).
 
 Tensors live on the GPU; every call is asynchronous on torch's current stream of the tensors' device and may be captured into a
-HIP graph.  There is no CPU path: a tensor elsewhere, or a shape or type a kernel does not cover, raises ``EngineError``."""
+HIP graph (group_norm_act's backward pass under the condition that stands there).  There is no CPU path: a tensor elsewhere, or a shape or type a kernel does not cover, raises ``EngineError``."""
 from __future__ import annotations
 
 import ctypes as C
@@ -125,9 +125,42 @@ def _norm_workspace(backward: int, n: int, hw: int, c: int, groups: int) -> int:
     return max(int(size), 16)
 
 
+# torch keeps one node per leaf (the one that accumulates its gradient) for as long as any autograd graph of the leaf lives, and the node keeps
+# the stream it was made under.  A backward pass under capture that meets a node made outside ties a stream outside the capture to the
+# captured one, which ends the process, not the call.  So every graph of group_norm_act is known by its leaves while it lives, and a
+# differentiable call under capture is refused where an eager graph shares one.
+class _Graph:
+    """held by the autograd node of one eager call: its leaves (ids of tensors that live as long as the node) stand in ``alive`` until it ends"""
+
+    __slots__ = ()
+    alive: dict = {}
+
+    def __init__(self, leaves):
+        self.alive[id(self)] = leaves
+
+    def __del__(self):
+        self.alive.pop(id(self), None)
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _enter_graph(tensors) -> _Graph | None:
+    """what the node of a call with these tensors holds; refuses a capture beside an eager graph of the same leaves"""
+    leaves = [id(t) for t in tensors if t.requires_grad and t.is_leaf] if torch.is_grad_enabled() else None
+    if not leaves:
+        return None
+    if not _capturing():
+        return _Graph(leaves)
+    if any(i in held for held in list(_Graph.alive.values()) for i in leaves):
+        raise EngineError("group_norm_act under graph capture: an eager autograd graph of the same parameters is alive; drop its outputs and losses first")
+    return None
+
+
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, groups, eps, act):
+    def forward(ctx, x, weight, bias, residual, groups, eps, act, graph):
         n, c, h, w = x.shape
         x = _dense(x)
         residual = _dense(residual) if residual is not None else None
@@ -143,7 +176,7 @@ class _GroupNormAct(torch.autograd.Function):
                 _NN_DTYPES[x.dtype], _NN_DTYPES[pd], n, h * w, c, groups, act, float(eps), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias),
                 _ptr(y), _ptr(stats), ws, size, _stream(x.device)))
         ctx.save_for_backward(x, weight, bias, residual, stats)
-        ctx.groups, ctx.act, ctx.pd = groups, act, pd
+        ctx.groups, ctx.act, ctx.pd, ctx.graph = groups, act, pd, graph
         return y
 
     @staticmethod
@@ -166,7 +199,7 @@ class _GroupNormAct(torch.autograd.Function):
                     _ptr(dy), _ptr(stats), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), size, _stream(x.device)))
         if need_r and dr is None:
             dr = dy  # (no activation: the sum passes the gradient on)
-        return dx, dw, db, dr, None, None, None
+        return dx, dw, db, dr, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
@@ -174,7 +207,12 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     """``act(group_norm(x) * weight + bias (+ residual))`` with its gradient, for x (N, C, H, W) f32 / bf16 / f16 whose memory is
     channels last (other layouts are copied into it first; the result is channels last).  ``activation``: "none", "relu" or
     "silu".  weight and bias (C,) are f32 or of x's dtype, both alike; ``residual`` is like x.  Statistics are held in f64, the
-    rest in f32, and each output is rounded once.  Differentiable once, in every tensor argument."""
+    rest in f32, and each output is rounded once.  Differentiable once, in every tensor argument.
+
+    Forward and backward may be captured into a HIP graph, the backward pass only while no eager autograd graph of the same leaves
+    (parameters) is alive: a kept output or loss of an eager step keeps its graph.  A differentiable call under capture raises
+    ``EngineError`` beside an eager graph of this operator's own that shares a leaf; graphs of the same leaves that run through other
+    operators alone are not seen, and capturing a backward pass beside one ends the process."""
     _on_gpu(x, "x", tuple(_NN_DTYPES))
     if x.dim() != 4:
         raise EngineError(f"x: expected (N, C, H, W), got {tuple(x.shape)}")
@@ -198,7 +236,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         _on_gpu(residual, "residual", (x.dtype,), x.device)
         if residual.shape != x.shape:
             raise EngineError(f"residual: expected {tuple(x.shape)}, got {tuple(residual.shape)}")
-    return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, ACTIVATIONS[activation])
+    graph = _enter_graph([t for t in (x, weight, bias, residual) if t is not None])
+    return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, ACTIVATIONS[activation], graph)
 
 
 @torch.no_grad()
