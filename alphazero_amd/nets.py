@@ -130,14 +130,16 @@ class GomokuNet(DualHeadNet):
 
     ``norm="group"``: every BatchNorm2d + ReLU becomes a GroupNormAct (``groups`` groups of the trunk's channels, one group in the
     heads).  Such a net has no running statistics: training and evaluation are one function, and the ranks of a data-parallel run
-    hold nothing that drifts apart between weight broadcasts.  It runs through its own forward (on the GPU, in channels-last memory),
-    not on the fused towers, which fold BatchNorm into their convolutions."""
+    hold nothing that drifts apart between weight broadcasts.  It runs through its own forward, on the GPU, not on the fused towers, which
+    fold BatchNorm into their convolutions.  Its input is laid out channels last first: the convolutions keep that layout, in which
+    the norms take their samples without a copy."""
 
     def __init__(self, board_size: int = 15, channels: int = 64, blocks: int = 2, history_len: int = HISTORY_LEN, norm: str = "batch",
                  groups: int = 8) -> None:
         super().__init__()
         a = board_size * board_size
         self.board_size = board_size
+        self._channels_last = norm == "group"
         if norm not in ("batch", "group"):
             raise ValueError("norm: 'batch' or 'group'")
         if norm == "group":
@@ -154,6 +156,9 @@ class GomokuNet(DualHeadNet):
                                           nn.Flatten(1), nn.Linear(a, a))
         self._value_head = nn.Sequential(nn.Conv2d(channels, 2, 1, bias=False), nn.BatchNorm2d(2), nn.ReLU(),
                                          nn.Flatten(1), *_mlp_value(2 * a))
+
+    def forward(self, x: torch.Tensor):
+        return super().forward(x.contiguous(memory_format=torch.channels_last) if self._channels_last else x)
 
     def flops_per_eval(self) -> float:
         """multiply-adds x2 of one forward (convs + linears), for MFMA utilisation reporting"""
