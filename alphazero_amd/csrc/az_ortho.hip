@@ -203,7 +203,7 @@ template <class T, int P, int PADT> __global__ __launch_bounds__(NT) void k_os_p
 
 // 1 KiB from memory to LDS: 16 bytes a lane, at lds + 16 lane
 __device__ __forceinline__ void to_lds(const char *base, uint32_t lane_off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
 }
 // all but the newest N of this wave's moves have landed and its LDS reads are done, then the workgroup goes on
 template <int N> __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory"); }
