@@ -8,11 +8,13 @@
 // Bound by bytes: forward reads x (and r) and writes y, backward reads x, dy (and r) and writes dx (and dr).  A large copy reaches 5.04 TB/s
 // on this card (reads and writes counted).  A sample whose channels fit a workgroup's registers is read once (k_gn_fwd_one, k_gn_bwd_one);
 // a larger one is shared out over workgroups and read twice.  Measured:
-//   1,024 x 128 x 15 x 15 f32, relu, residual: forward 76.7 us (354 MB: 4.6 TB/s), backward 117.8 us (590 MB: 5.0 TB/s) + 5.5 us for dw, db
-//   16,384 x 64 x 15 x 15 bf16, relu, forward: 162 us (944 MB: 5.8 TB/s)
-//   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.4 + 4.0 + 23.4 us, backward 26.4 + 4.9 + 33.4 + 4.2 us (66.6 MB a tensor: the four
-//                                              passes move 5.0, 5.7, 5.0 and 6.0 TB/s)
-//   64 x 64 x 9 x 9 f32, relu:                 4.2 us, 4.7 + 3.0 us; the call is bound by the host (112 us with autograd's own 72)
+//   1,024 x 128 x 15 x 15 f32, relu, residual: forward 77.5 us (354 MB: 4.6 TB/s), backward 117.5 us (590 MB: 5.0 TB/s) + 5.5 us for dw, db
+//   16,384 x 64 x 15 x 15 bf16, relu, forward: 164 us (944 MB: 5.8 TB/s)
+//   4 x 512 x 128 x 127 f16, silu, in chunks:  forward 13.9 + 4.4 + 22.9 us, backward 26.8 + 5.0 + 33.2 + 4.0 us (66.6 MB a tensor: the four
+//                                              passes move 4.8, 5.8, 5.0 and 6.0 TB/s)
+//   64 x 64 x 9 x 9 f32, relu:                 4.3 us, 4.8 + 3.1 us; the call is bound by the host (113 .. 120 us with autograd's own 72)
+//   Slower than they could be (a group's vectors no power of two: in chunks; one or two channels: single elements, and one thread a group adds up):
+//   1,024 x 192 x 15 x 15 f32 in 8 groups, relu: 314 us forward and backward; 16,384 x 1 x 15 x 15 bf16 forward 277 us (a floor of 3)
 // Mean and variance come from f64 sums of x - p and (x - p)^2 in one pass, p the group's first value (of the sample's first pixel).  p is one
 // of the m values, so (mean - p)^2 <= m var: the sums lose at most a factor of m of f64's 53 bits wherever the values lie (sums of x and x^2
 // lose (mean / deviation)^2 of them), and a flat group has no variance at all.  The mean is kept as a pair of f32 for the subtraction,

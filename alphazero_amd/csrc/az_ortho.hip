@@ -19,11 +19,12 @@
 // pieces lie at piece ^ (r & 7), so that the 8 rows a quarter wave reads at once fall on different banks.
 //
 // Measured (a large f16 product by the library reaches 1,116 TFLOP/s on this card, a bf16 one 1,169):
-//   4096 x 4096 bf16:                  1.73 ms; X 155 .. 159 us (137 GFLOP: 0.87 PFLOP/s), A and B 96 and 98 us (half of that: 0.72)
-//   2501 x 1203 f32:                   424 us; X 42 us (22.2 GFLOP executed in three products of halves: 0.53 PFLOP/s): 1.5 tiles a slot
-//   the deep 128-channel net's 23 f32: 179 us in 22 launches: 13 us for X (4.7 GFLOP executed), 9 + 5 for A, 6 for B: launches, and 752 tiles of
+//   4096 x 4096 bf16:                  1.74 ms; X 154 .. 166 us (137 GFLOP: 0.87 PFLOP/s), A and B 92 and 96 us (half of that: 0.73)
+//   2501 x 1203 f32:                   451 us; X 42 us (22.2 GFLOP executed in three products of halves: 0.53 PFLOP/s): 1.5 tiles a slot
+//   the deep 128-channel net's 23 f32: 183 us in 22 launches: 13 us for X (4.7 GFLOP executed), 9 + 5 for A, 6 for B: launches, and 752 tiles of
 //                                      4 stages each, whose start and end weigh as much as their products
-//   64 x 576 f32:                      54 us in one launch, 11 a step: latencies of one workgroup (below)
+//   1536 x 1536 bf16 / f32:            260 / 489 us; 2000 x 4096 bf16 / f32: 615 / 1,348 us
+//   64 x 576 f32 or bf16:              54 us in one launch, 11 a step: latencies of one workgroup (below)
 #include "az_ops.hip.h"
 
 #include <cmath>
@@ -673,7 +674,7 @@ static bool is_small(int rows, int cols) {
 // f16 halves a factor is held in.  bf16 matrices with a short side beyond 64 make do with one: the errors of 11-bit factors, beside the 8-bit result's own
 // rounding of 1.66e-3 (relative, Frobenius), come to 2.0e-3 .. 2.8e-3 in all (4096 x 4096 1.98e-3; short sides of 80 to 200 the most).  On short sides
 // of 64 and less there are too few directions for them to average out (64 x 576 4.1e-3, 1 x 7 6.3e-3), and a second half costs little (64 x 576 alone
-// 34 -> 55 us; 1536 x 1536 would take 470 instead of 250).
+// 34 -> 55 us; 1536 x 1536 would take 480 instead of 260).
 static int planes_of(int32_t dtype, int rows, int cols) { return dtype == AZ_NN_BF16 && (rows < cols ? rows : cols) > SMALL_S ? 1 : 2; }
 
 static int64_t round_up(int64_t v) { return (v + 255) / 256 * 256; }

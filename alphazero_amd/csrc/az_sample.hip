@@ -19,12 +19,17 @@
 //               the prefix ends within the list, the rest is done on it.  A longer prefix is found from a histogram linear in the
 //               score and a list of the bin it ends in.
 //
-// Bound by instructions: about ten a score and walk, and 25 f64 operations an exponential where the kept scores are many.  Measured:
+// Bound by instructions and, in long rows, by latencies: about ten instructions a score and walk, and 25 f64 operations an exponential where the
+// kept scores are many.  Measured (long rows: scores of deviation 3):
 //   16,384 x 225 f32, masks, top k 16, top p 0.9, min p:   37 us (20.6 k vector instructions a SIMD, 34 us at four cycles each; the 18.6 MB
 //                                                          would take 3.7)
 //   1 x 225 f32:                                           5.4 us, the latency of one wave's steps; the call 12 us
-//   512 x 65,537 bf16, top p 0.9, min p:                   93 us (67 MB: 0.72 TB/s)
-//   1 x 131,072 bf16, top k 50, top p 0.95:                38 us on one CU: a row is not shared out, its sums and lists stay in LDS
+//   512 x 65,537 bf16, T 0.7, top p 0.9, min p:            93 us (67 MB, read twice: 1.4 TB/s; 22.1 k vector instructions a SIMD take 37 us of it, and two waves
+//                                                          a SIMD do not cover the walks' loads and the list's steps between barriers)
+//     T 1, top p 0.9:                                      250 us: the prefix has more than 1,024 members, the list overflows, and of six walks two
+//                                                          take an f64 exponential of every score
+//     T 0.8, top k 50, top p 0.95 / T 1, no cut:           48 / 80 us
+//   1 x 131,072 bf16, T 0.8, top k 50, top p 0.95:         38 us on one CU: a row is not shared out, its sums and lists stay in LDS; T 1, top p 0.9: 196 us
 #include "az_ops.hip.h"
 
 namespace azsample {

@@ -75,6 +75,8 @@ def sample_actions(scores: torch.Tensor, uniforms: torch.Tensor, *, temperature=
     temperature 0 takes the first of the largest.  ``legal`` (rows, n) bool: scores outside it, NaN and -inf do not count; scores
     of +inf share the whole mass.  temperature, top_p, min_p (f32) and top_k (i32) may be tensors of (rows,).
 
+    Not differentiable: the log-probability carries no autograd graph, whether the scores require a gradient or not.
+
     For moves from a search: scores = log(visits) makes the weights visits ** (1 / temperature) (training/self_play.py:73-74)."""
     _on_gpu(scores, "scores", tuple(_NN_DTYPES))
     if scores.dim() != 2 or scores.shape[1] < 1 or scores.shape[1] > 524288 or scores.shape[0] > 0x7FFFFFFF:
