@@ -128,9 +128,10 @@ def _norm_workspace(backward: int, n: int, hw: int, c: int, groups: int) -> int:
 
 
 # torch keeps one node per leaf (the one that accumulates its gradient) for as long as any autograd graph of the leaf lives, and the node keeps
-# the stream it was made under.  A backward pass under capture that meets a node made outside ties a stream outside the capture to the
-# captured one, which ends the process, not the call.  So every graph of group_norm_act is known by its leaves while it lives, and a
-# differentiable call under capture is refused where an eager graph shares one.
+# the stream it was made under: a backward pass hands gradients over to that stream and waits for it.  Under capture a side stream is drawn
+# into the capture by that and joined again; the default stream may not take part in one (torch's warning of a mismatched stream
+# of such a node says as much), and the error ends the process, not the call.  So every graph of group_norm_act whose leaves' nodes may be the default stream's is known by its leaves while it lives, and a differentiable
+# call under capture is refused where such a graph shares a leaf.
 class _Graph:
     """held by the autograd node of one eager call: its leaves (ids of tensors that live as long as the node) stand in ``alive`` until it ends"""
 
@@ -143,20 +144,30 @@ class _Graph:
     def __del__(self):
         self.alive.pop(id(self), None)
 
+    @classmethod
+    def holds(cls, leaves) -> bool:
+        return any(i in held for held in list(cls.alive.values()) for i in leaves)
+
 
 def _capturing() -> bool:
     return torch.cuda.is_current_stream_capturing()
 
 
+def _on_default_stream(device: torch.device) -> bool:
+    return torch._C._cuda_getCurrentRawStream(device.index) == 0
+
+
 def _enter_graph(tensors) -> _Graph | None:
-    """what the node of a call with these tensors holds; refuses a capture beside an eager graph of the same leaves"""
+    """what the node of a call with these tensors holds; refuses a capture beside an eager default-stream graph of the same leaves"""
     leaves = [id(t) for t in tensors if t.requires_grad and t.is_leaf] if torch.is_grad_enabled() else None
     if not leaves:
         return None
     if not _capturing():
-        return _Graph(leaves)
-    if any(i in held for held in list(_Graph.alive.values()) for i in leaves):
-        raise EngineError("group_norm_act under graph capture: an eager autograd graph of the same parameters is alive; drop its outputs and losses first")
+        # (on a side stream too, beside a graph that is known: it shares that one's nodes, and may outlive it)
+        return _Graph(leaves) if _on_default_stream(tensors[0].device) or _Graph.holds(leaves) else None
+    if _Graph.holds(leaves):
+        raise EngineError("group_norm_act under graph capture: an eager autograd graph of the same parameters, made on the default stream, is alive; "
+                          "drop its outputs and losses first, or make it on a side stream")
     return None
 
 
@@ -212,9 +223,10 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     rest in f32, and each output is rounded once.  Differentiable once, in every tensor argument.
 
     Forward and backward may be captured into a HIP graph, the backward pass only while no eager autograd graph of the same leaves
-    (parameters) is alive: a kept output or loss of an eager step keeps its graph.  A differentiable call under capture raises
-    ``EngineError`` beside an eager graph of this operator's own that shares a leaf; graphs of the same leaves that run through other
-    operators alone are not seen, and capturing a backward pass beside one ends the process."""
+    (parameters) that was made on the default stream is alive: a kept output or loss of such a step keeps its graph.  A differentiable
+    call under capture raises ``EngineError`` beside such a graph of this operator's own that shares a leaf; graphs of the same leaves that
+    run through other operators alone are not seen, and capturing a backward pass beside one ends the process.
+    ``torch.cuda.make_graphed_callables``, which warms up on a side stream, works."""
     _on_gpu(x, "x", tuple(_NN_DTYPES))
     if x.dim() != 4:
         raise EngineError(f"x: expected (N, C, H, W), got {tuple(x.shape)}")

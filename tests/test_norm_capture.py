@@ -1,5 +1,5 @@
-"""A graph capture is refused while an eager autograd graph of the same leaves lives (its backward pass would end the process).  Nothing is
-captured here: the stream is said to be capturing."""
+"""A differentiable call under graph capture is refused while an eager autograd graph of the same leaves lives that was made on the default
+stream (the captured backward pass would end the process).  Where that is tested nothing is captured: the stream is said to be capturing."""
 import gc
 
 import pytest
@@ -23,8 +23,9 @@ def test_a_leaf_is_held_as_long_as_its_graph(monkeypatch):
     from alphazero_amd import ops
     from alphazero_amd.engine import EngineError
 
-    capturing = [False]
+    capturing, default = [False], [True]
     monkeypatch.setattr(ops, "_capturing", lambda: capturing[0])
+    monkeypatch.setattr(ops, "_on_default_stream", lambda device: default[0])
     x, w, other = torch.ones(3), torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
 
     def enter(*ts):
@@ -57,7 +58,21 @@ def test_a_leaf_is_held_as_long_as_its_graph(monkeypatch):
     assert not refused(w)
     hidden = w * 1  # not a leaf
     assert enter(hidden) is None
-    del y
+    del y, hidden
+    default[0] = False
+    side = _Node.apply(x, w, enter(x, w))  # nor does one made on a side stream,
+    assert not refused(w)
+    del side
+    default[0] = True
+    first = _Node.apply(x, w, enter(x, w))
+    default[0] = False
+    side = _Node.apply(x, w, enter(x, w))  # but for one that shares the node of a default-stream graph, which it keeps
+    del first
+    gc.collect()
+    assert refused(w)
+    del side
+    gc.collect()
+    assert not refused(w)
 
 
 @pytest.mark.gpu
@@ -81,3 +96,26 @@ def test_group_norm_act_refuses_and_goes_on(monkeypatch):
     y = norm(x)
     assert torch.equal(y, want)
     y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_make_graphed_callables():
+    """forward and backward captured by torch's own means, which keeps the graph of its warm-up on a side stream"""
+    from alphazero_amd.nets import GroupNormAct
+
+    torch.manual_seed(0)
+    norm = GroupNormAct(2, 8).cuda()
+    plain = GroupNormAct(2, 8).cuda()
+    last = lambda t: t.contiguous(memory_format=torch.channels_last)
+    graphed = torch.cuda.make_graphed_callables(norm, (last(torch.randn(4, 8, 9, 9, device="cuda")).requires_grad_(True),))
+    for seed in range(3):
+        x = last(torch.randn(4, 8, 9, 9, device="cuda")).requires_grad_(True)
+        xp = x.detach().clone().requires_grad_(True)
+        dy = last(torch.randn(4, 8, 9, 9, device="cuda"))
+        y, yp = graphed(x), plain(xp)
+        assert torch.equal(y, yp)
+        got = torch.autograd.grad(y, [x, *norm.parameters()], dy)
+        want = torch.autograd.grad(yp, [xp, *plain.parameters()], dy)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del y, yp, got, want
