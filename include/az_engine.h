@@ -492,9 +492,10 @@ int az_group_norm_backward(int32_t dtype, int32_t param_dtype, int64_t n, int64_
  * 1.2 .. 1.7 times the error of the result's own rounding in all).  Entries of X below 2^-16 keep fewer bits (they stand in steps of 2^-38 with the
  * usual coefficients): a matrix whose norm is far below eps loses accuracy.  A matrix with an infinity or a NaN gives NaN, a zero matrix
  * zeros.  Coefficients under which a singular value in [0, 1] could grow beyond 7.5 are refused.
- * A matrix's result does not depend on the others of the call, but for matrices of at most 64 x 768: beside a larger one (of bf16 matrices:
- * beside a longer one with a short side of at most 64) they take another kernel, whose sums run in another order.  Either result is as exact as
- * said above, and they differ by as much (64 x 576 f32: by up to 2e-6 of the result's norm, the error of either).
+ * A matrix's result does not depend on the others of the call, but for matrices of at most 64 x 768: beside a larger one that shares their
+ * launches (f32 and f16: a short side below 1,792; bf16: a short side of at most 64) they take another kernel, whose sums run in another
+ * order.  Either result is as exact as said above, and they differ by as much (64 x 576 f32: by up to 2e-6 of the result's norm, the error of
+ * either).
  * workspace_dev: az_orthogonalize_workspace() bytes (0: none; -1: refused), aligned to 256 bytes, meaningless between calls; calls that overlap in
  * time need one each. */
 int64_t az_orthogonalize_workspace(int32_t dtype, int32_t count, const int32_t *rows, const int32_t *cols);

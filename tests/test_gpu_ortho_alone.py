@@ -102,3 +102,16 @@ def test_buffers_that_start_beyond_4_gib():
     one = ops.orthogonalize(m, steps=1)
     for o in ops.orthogonalize([m, m, m], steps=1):
         assert torch.equal(o, one)
+
+
+@pytest.mark.parametrize("dtype,other", [(torch.float32, (1800, 1900)), (torch.float16, (1800, 1900)), (torch.bfloat16, (100, 900)), (torch.bfloat16, (1800, 1900))], ids=str)
+def test_small_matrices_beside_those_that_share_no_launch(dtype, other):
+    """a larger matrix of another tile size, or of another number of halves, leaves the small ones their own kernel: nothing changes, bit for bit"""
+    from alphazero_amd import ops
+
+    small = [make(s, dtype, i, 0.01) for i, s in enumerate(((64, 576), (20, 700), (1, 7), (33, 32), (768, 64)))]
+    larger = make(other, dtype, 90)
+    got = ops.orthogonalize([small[0], larger, *small[1:]])
+    assert torch.equal(got[1], ops.orthogonalize(larger))
+    for o, alone in zip([got[0], *got[2:]], ops.orthogonalize(small)):
+        assert torch.equal(o, alone)
