@@ -134,15 +134,17 @@ class GomokuNet(DualHeadNet):
     fold BatchNorm into their convolutions.  Its input is laid out channels last first: the convolutions keep that layout, in which
     the norms take their samples without a copy."""
 
+    _channels_last = False  # (of the class, for nets that were saved whole before there was a choice of norms)
+
     def __init__(self, board_size: int = 15, channels: int = 64, blocks: int = 2, history_len: int = HISTORY_LEN, norm: str = "batch",
                  groups: int = 8) -> None:
         super().__init__()
         a = board_size * board_size
         self.board_size = board_size
-        self._channels_last = norm == "group"
         if norm not in ("batch", "group"):
             raise ValueError("norm: 'batch' or 'group'")
         if norm == "group":
+            self._channels_last = True
             self._shared_layers = nn.Sequential(
                 nn.Conv2d(history_len + 1, channels, 3, padding=1, bias=False), GroupNormAct(groups, channels),
                 *[_GroupRes(channels, groups) for _ in range(blocks)])
